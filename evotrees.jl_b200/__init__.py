@@ -13,4 +13,13 @@ from ._lib import EvbError, trim_cache
 
 __all__ = ["trim_cache", "EvoTreeRegressor", "EvoTreeClassifier", "EvoTreeMLE", "EvoTreeCount", "EvoTypes", "EvoTree", "Tree", "predict",
            "predict_leaf_idx", "predict_binned", "fit", "init_core", "init_core_binned", "grow_evotree", "grow_tree", "grow_tree_begin", "grow_tree_end", "grow_rounds", "sample_round",
-           "Cache", "CallBack", "init_logger", "update_logger", "eval_levelcode", "IS_MAXIMISE", "binarize", "get_edges", "EvbError"]
+           "Cache", "CallBack", "init_logger", "update_logger", "eval_levelcode", "IS_MAXIMISE", "binarize", "get_edges", "distill_grads", "policy_grads",
+           "preference_grads", "EvbError"]
+
+
+def __getattr__(name):      # these take torch tensors: the rest of the package does without importing torch
+    if name in ("distill_grads", "policy_grads", "preference_grads"):
+        from . import losses
+        globals()[name] = getattr(losses, name)
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

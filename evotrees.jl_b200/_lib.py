@@ -13,7 +13,7 @@ import numpy as np
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libevotrees_b200.so")
 
-EVB_F32, EVB_U32, EVB_F64 = 0, 1, 2
+EVB_F32, EVB_U32, EVB_F64, EVB_BF16, EVB_F16 = 0, 1, 2, 3, 4
 ERR_LIMIT, ERR_STALE = -7, -8
 LOSS_CODES = {"mse": 0, "logloss": 1, "mlogloss": 2, "gaussian_mle": 3, "poisson": 4, "gamma": 5, "tweedie": 6, "logistic_mle": 7,
               "mae": 8, "cred_var": 9, "cred_std": 10, "quantile": 11, "multiquantile": 12}
@@ -27,7 +27,8 @@ TIMER_NAMES = ["grads", "rows_init", "hist", "hist_reduce", "allreduce", "scan",
 EXPORTS = ["evb_last_error", "evb_version", "evb_create", "evb_create_x", "evb_create_m", "evb_matrix_create", "evb_matrix_edges", "evb_matrix_destroy",
            "evb_eval_attach_m", "evb_host_range", "evb_host_count", "evb_host_codes", "evb_host_std", "evb_destroy", "evb_comm_unique_id", "evb_comm_init", "evb_comm_ipc_export", "evb_comm_ipc_import",
            "evb_grow_tree", "evb_grow_tree_begin", "evb_grow_tree_begin_pcg", "evb_grow_tree_end", "evb_eval_attach", "evb_eval_sums", "evb_eval_get_pred", "evb_eval_detach", "evb_test_peer_timeout", "evb_test_grid_timeout", "evb_test_quotients", "evb_test_predict_plan", "evb_set_timing", "evb_get_pred", "evb_get_grads", "evb_get_nidx", "evb_get_hist", "evb_get_node_sums",
-           "evb_get_stream", "evb_get_timings", "evb_reset_timings", "evb_predict", "evb_predict_x", "evb_model_create", "evb_model_predict", "evb_model_destroy", "evb_binarize", "evb_hist_rows", "evb_hist_rows_noalloc", "evb_trim_cache"]
+           "evb_get_stream", "evb_get_timings", "evb_reset_timings", "evb_predict", "evb_predict_x", "evb_model_create", "evb_model_predict", "evb_model_destroy", "evb_binarize", "evb_hist_rows", "evb_hist_rows_noalloc", "evb_distill_grads", "evb_policy_grads",
+           "evb_preference_grads", "evb_trim_cache"]
 
 
 class EvbError(RuntimeError):
@@ -68,6 +69,11 @@ def lib() -> C.CDLL:
         # declared: plain integers are then passed without a wrapper object per argument (a call with one row takes ~20 us)
         _lib.evb_model_predict.argtypes = [C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_int32, C.c_void_p,
                                            C.c_void_p, C.c_void_p]
+        i4, i8, f8, ptr_ = C.c_int32, C.c_int64, C.c_double, C.c_void_p
+        rows = [i4, ptr_, ptr_, i4, i8, i4, i8]
+        _lib.evb_distill_grads.argtypes = rows + [ptr_, ptr_, i4, i4, i4, ptr_, f8, ptr_, ptr_, i8, ptr_, i8]
+        _lib.evb_policy_grads.argtypes = rows + [ptr_, ptr_, ptr_, ptr_, ptr_, f8, f8, f8, f8, ptr_, ptr_, ptr_, i8, ptr_, i8]
+        _lib.evb_preference_grads.argtypes = rows + [ptr_, ptr_, i4, ptr_, ptr_, f8, f8, i4, ptr_, ptr_, ptr_, ptr_, i8, ptr_]
     return _lib
 
 

@@ -1,0 +1,110 @@
+"""Losses on rows of raw predictions that live on the GPU, with their gradients (and hessians, for boosting): distillation from a
+teacher's top logits, the clipped policy loss with a KL term, the preference loss of paired log ratios.  The formulas are in
+include/evb.h (`evb_distill_grads`, `evb_policy_grads`, `evb_preference_grads`).
+
+Arrays are torch tensors on one CUDA device.  `pred` is [rows, classes] float32, bfloat16 or float16, a row's classes side by side, rows at
+any stride; class codes are int32, 1..classes, 0 = none.  Per-row vectors are contiguous float32.  Calls run on the device's current
+stream, wait for nothing, and can be captured into a CUDA graph; they take no part in autograd: gradients are returned.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.EVB_F32, torch.bfloat16: _lib.EVB_BF16, torch.float16: _lib.EVB_F16}
+
+
+def _rows(pred):
+    """Type code, rows, classes and row stride of `pred`."""
+    if not isinstance(pred, torch.Tensor) or pred.dim() != 2:
+        raise ValueError("`pred` must be a torch tensor of shape [rows, classes]")
+    code = _DTYPES.get(pred.dtype)
+    if code is None:
+        raise ValueError(f"`pred` must be float32, bfloat16 or float16, not {pred.dtype}")
+    if not pred.is_cuda:
+        raise _lib.EvbError(-2, "`pred` is not on a CUDA device: this library has no CPU fallback")
+    n, K = pred.shape
+    if K < 1:
+        raise ValueError("`pred` has no classes")
+    ld = pred.stride(0) if n > 1 else K
+    if (K > 1 and pred.stride(1) != 1) or ld < K:
+        raise ValueError("the classes of a row of `pred` must lie side by side, rows behind one another")
+    return code, n, K, ld
+
+
+def _vec(name, v, shape, dtype, pred):
+    """Address of an array that goes with `pred`."""
+    if not isinstance(v, torch.Tensor) or v.dtype is not dtype or v.shape != shape or v.device != pred.device or not v.is_contiguous():
+        raise ValueError(f"`{name}` must be a contiguous {dtype} tensor of shape {list(shape)} on {pred.device}")
+    return v.data_ptr()
+
+
+def _stream(pred):
+    return torch.cuda.current_stream(pred.device).cuda_stream
+
+
+def distill_grads(pred, ids, teacher, *, w=None, tau: float = 1.0, tail: bool = False, hess: bool = False, grads: bool = True):
+    """Divergence from a teacher of whom the top classes of every row were kept: `ids` int32 [rows, slots] (0 = empty) with `teacher`
+    [rows, slots], its logits, or with `tail=True` its log-probabilities, the probability of all other classes then being one class
+    more.  Returns (loss [rows], gradient [rows, classes][, hessian]); the loss alone with `grads=False`."""
+    code, n, K, ld = _rows(pred)
+    if not isinstance(ids, torch.Tensor) or ids.dim() != 2 or ids.shape[1] < 1:
+        raise ValueError("`ids` must be a torch tensor of shape [rows, slots] with at least one slot")
+    shape = torch.Size((n, ids.shape[1]))
+    pi = _vec("ids", ids, shape, torch.int32, pred)
+    tcode = _DTYPES.get(getattr(teacher, "dtype", None))
+    if tcode is None:
+        raise ValueError("`teacher` must be a float32, bfloat16 or float16 tensor")
+    pt = _vec("teacher", teacher, shape, teacher.dtype, pred)
+    pw = None if w is None else _vec("w", w, shape[:1], torch.float32, pred)
+    loss = torch.empty(n, dtype=torch.float32, device=pred.device)
+    g = torch.empty((n, K), dtype=pred.dtype, device=pred.device) if grads else None
+    h = torch.empty((n, K), dtype=pred.dtype, device=pred.device) if grads and hess else None
+    _lib.check(_lib.lib().evb_distill_grads(pred.device.index, _stream(pred), pred.data_ptr(), code, n, K, ld, pi, pt, tcode, shape[1], bool(tail), pw,
+                                            tau, loss.data_ptr(), None if g is None else g.data_ptr(), K, None if h is None else h.data_ptr(), K))
+    return (loss,) if g is None else (loss, g) if h is None else (loss, g, h)
+
+
+def policy_grads(pred, action, old_logp, adv, *, ref_logp=None, w=None, tau: float = 1.0, clip=(0.2, 0.2), beta: float = 0.0,
+                 hess: bool = False, grads: bool = True):
+    """Clipped policy loss of the class `action` (int32 [rows], 0 = the row does not count) that was taken with log-probability `old_logp`
+    and turned out with advantage `adv`, plus `beta` times an estimate of the divergence from a reference policy (`ref_logp`).
+    Returns (loss [rows], logp [rows], gradient [rows, classes][, hessian]); (loss, logp) with `grads=False`."""
+    code, n, K, ld = _rows(pred)
+    row = torch.Size((n,))
+    pa = _vec("action", action, row, torch.int32, pred)
+    po, pv = _vec("old_logp", old_logp, row, torch.float32, pred), _vec("adv", adv, row, torch.float32, pred)
+    pr = None if ref_logp is None else _vec("ref_logp", ref_logp, row, torch.float32, pred)
+    pw = None if w is None else _vec("w", w, row, torch.float32, pred)
+    low, high = clip
+    loss, logp = torch.empty((2, n), dtype=torch.float32, device=pred.device)
+    g = torch.empty((n, K), dtype=pred.dtype, device=pred.device) if grads else None
+    h = torch.empty((n, K), dtype=pred.dtype, device=pred.device) if grads and hess else None
+    _lib.check(_lib.lib().evb_policy_grads(pred.device.index, _stream(pred), pred.data_ptr(), code, n, K, ld, pa, po, pv, pr, pw, tau, low, high, beta,
+                                           loss.data_ptr(), logp.data_ptr(), None if g is None else g.data_ptr(), K, None if h is None else h.data_ptr(), K))
+    return (loss, logp) if g is None else (loss, logp, g) if h is None else (loss, logp, g, h)
+
+
+def preference_grads(pred, label, seq, *, ref_logp=None, w=None, beta: float = 0.1, smooth: float = 0.0, mean: bool = False, grads: bool = True):
+    """Preference loss of pairs of sequences of rows.  `label` int32 [rows] is the class of every row (0 = not counted), `seq` int32
+    [2 pairs + 1] where the sequences begin and end: sequence 2 p is preferred to sequence 2 p + 1.  The margin of a pair is `beta` times
+    the difference of the sequences' sums (`mean=True`: means) of log p - `ref_logp`.
+    Returns (loss [pairs], margin [pairs], logp [rows], gradient [rows, classes]); without the last with `grads=False`."""
+    code, n, K, ld = _rows(pred)
+    row = torch.Size((n,))
+    pl = _vec("label", label, row, torch.int32, pred)
+    if not isinstance(seq, torch.Tensor) or seq.dim() != 1 or seq.shape[0] % 2 != 1:
+        raise ValueError("`seq` must be a torch tensor of 2 pairs + 1 row numbers")
+    P = seq.shape[0] // 2
+    ps = _vec("seq", seq, seq.shape, torch.int32, pred)
+    pr = None if ref_logp is None else _vec("ref_logp", ref_logp, row, torch.float32, pred)
+    pw = None if w is None else _vec("w", w, torch.Size((P,)), torch.float32, pred)
+    loss, margin = torch.empty((2, P), dtype=torch.float32, device=pred.device)
+    logp = torch.empty(n, dtype=torch.float32, device=pred.device)
+    work = torch.empty(12 * n, dtype=torch.uint8, device=pred.device)
+    g = torch.empty((n, K), dtype=pred.dtype, device=pred.device) if grads else None
+    _lib.check(_lib.lib().evb_preference_grads(pred.device.index, _stream(pred), pred.data_ptr(), code, n, K, ld, pl, ps, P, pr, pw, beta, smooth,
+                                               bool(mean), loss.data_ptr(), margin.data_ptr(), logp.data_ptr(), None if g is None else g.data_ptr(), K,
+                                               work.data_ptr()))
+    return (loss, margin, logp) if g is None else (loss, margin, logp, g)

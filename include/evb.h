@@ -55,7 +55,7 @@ enum evb_loss { EVB_MSE = 0, EVB_LOGLOSS = 1, EVB_MLOGLOSS = 2, EVB_GAUSSIAN_MLE
                 EVB_MAE = 8, EVB_CRED_VAR = 9, EVB_CRED_STD = 10, EVB_QUANTILE = 11,
                 EVB_MULTIQUANTILE = 12 /* one target, K = number of quantiles evb_params.alphas[0..K-1], K <= 8 (src/loss.jl:160-172) */ };
 #define EVB_LOSS_LAST EVB_MULTIQUANTILE
-enum evb_dtype { EVB_F32 = 0, EVB_U32 = 1, EVB_F64 = 2 };
+enum evb_dtype { EVB_F32 = 0, EVB_U32 = 1, EVB_F64 = 2, EVB_BF16 = 3, EVB_F16 = 4 /* the last two: predictions of evb_*_grads only */ };
 
 /* flags of evb_params.flags */
 #define EVB_FLAG_TIMING 1u         /* record a CUDA-event pair (and an NVTX range) around every kernel class (see evb_get_timings) */
@@ -389,6 +389,59 @@ EVB_API int32_t evb_hist_rows(int32_t device, void *stream, const uint8_t *x_row
 EVB_API int32_t evb_hist_rows_noalloc(int32_t device, void *stream, const uint8_t *x_rows, int64_t nobs, int32_t nfeats,
                                       int32_t row_stride, int32_t nbins, const float *grad, int32_t nch, const uint32_t *rows,
                                       int64_t nrows, double *out);
+
+/*
+ * evb_distill_grads, evb_policy_grads, evb_preference_grads -- losses on rows of raw predictions that a softmax turns into probabilities,
+ * with their gradients, on buffers that already live on the device (no counterpart in the reference).
+ *   z        device, EVB_F32 / EVB_BF16 / EVB_F16, row i at z + i * ldz, K <= 1048576 classes; x = z / tau, lse = log sum_k e^x_k,
+ *            p = e^(x - lse)
+ *   w        device float [n] row weights, or NULL for ones.  A row of weight 0 counts for nothing, whatever else it holds: loss, gradient
+ *            and hessian are zeros there
+ *   loss     device float [n], or NULL (preferences: [pairs]); already multiplied by the weight
+ *   grad     device, type of z, row i at grad + i * ldg, or NULL: derivatives of the sum of the losses by z.  All K entries of all n rows
+ *            are written.  It must not overlap z
+ *   hess     the same for the second derivatives' positive part: w p_k (1 - p_k), divided by tau^2 for the policy loss; or NULL
+ *   class codes are 1..K; 0 names no class.  A row that names a class above K gets NaN in all its outputs.
+ * The calls enqueue their kernels on `stream` (cudaStream_t) and return; they allocate nothing and can be captured into a CUDA graph.  The
+ * calling thread's current device stays what it was.  Sums and probabilities are 32-bit floats whatever the type of z, sums of log
+ * ratios 64-bit ones; results do not depend on scheduling: equal calls give equal bits.
+ *
+ * evb_distill_grads -- Kullback-Leibler divergence from a teacher of whom T classes a row were kept.
+ *   ids      device uint32 [n][T] class codes, 0 = empty slot;  teacher  device [n][T], own type; a slot that holds -inf is empty too.
+ *            1 <= T <= 1024.  Rows without slots count for nothing.  A class in several slots counts with each of them.
+ *   tail=0   teacher holds logits: q_j = e^(t_j / tau) / sum, over the slots
+ *            loss = w tau^2 sum_j q_j (log q_j - log p_j),  grad_k = w tau (p_k - sum of q_j of class k)
+ *   tail=1   (tau = 1) teacher holds log-probabilities: q_j = e^t_j; the rest q_T = max(0, 1 - sum_j q_j) is compared with the
+ *            probability p_T of all classes that have no slot (q_T = 0 when there are none, or all of them are -inf); Q = sum_j q_j + q_T
+ *            loss = w (sum_j q_j (t_j - log p_j) + q_T (log q_T - log p_T))
+ *            grad_k = w (Q p_k - sum of q_j of class k), and w (Q p_k - q_T p_k / p_T) for classes without a slot
+ *
+ * evb_policy_grads -- clipped policy loss with a KL term, for the class (action) a that was taken.
+ *   action, old_logp, adv, ref_logp   device [n]; ref_logp NULL: no KL term.  action 0: the row counts for nothing
+ *            lp = log p_a,  r = e^(lp - old_logp),  x = ref_logp - lp
+ *            loss = w (-min(r adv, clamp(r, 1 - clip_low, 1 + clip_high) adv) + beta (e^x - x - 1))
+ *            d = -r adv where the minimum is the first of the two, else 0;  d += beta (1 - e^x);  grad_k = w d ([k = a] - p_k) / tau
+ *   logp     device float [n]: lp, or NULL
+ *
+ * evb_preference_grads -- preferences between sequences of rows by their log ratios.
+ *   label    device uint32 [n]: the class of every row, 0 = not counted (a prompt, padding)
+ *   seq      device int32 [2 pairs + 1] ascending within 0..n: sequence s is rows seq[s] .. seq[s + 1] - 1; pair p prefers sequence 2 p to
+ *            sequence 2 p + 1.  Rows outside of all sequences have zero gradients
+ *   ref_logp device float [n]: the reference's log-probabilities, or NULL for zeros;  w  device float [pairs] or NULL
+ *            D_s = sum over its rows of (log p_label - ref_logp), divided by their number when mean != 0;  m = beta (D_2p - D_2p+1)
+ *            loss = w ((1 - smooth) softplus(-m) + smooth softplus(m));  grad as it follows from that (tau = 1)
+ *   margin   device float [pairs]: m;  logp  device float [n]: log p_label, 0 where not counted
+ *   work     device, 12 n bytes, 8-byte aligned, in use until the call's kernels are done
+ */
+EVB_API int32_t evb_distill_grads(int32_t device, void *stream, const void *z, int32_t dtype, int64_t n, int32_t K, int64_t ldz, const uint32_t *ids,
+                                  const void *teacher, int32_t teacher_dtype, int32_t T, int32_t tail, const float *w, double tau, float *loss,
+                                  void *grad, int64_t ldg, void *hess, int64_t ldh);
+EVB_API int32_t evb_policy_grads(int32_t device, void *stream, const void *z, int32_t dtype, int64_t n, int32_t K, int64_t ldz, const uint32_t *action,
+                                 const float *old_logp, const float *adv, const float *ref_logp, const float *w, double tau, double clip_low,
+                                 double clip_high, double beta, float *loss, float *logp, void *grad, int64_t ldg, void *hess, int64_t ldh);
+EVB_API int32_t evb_preference_grads(int32_t device, void *stream, const void *z, int32_t dtype, int64_t n, int32_t K, int64_t ldz, const uint32_t *label,
+                                     const int32_t *seq, int32_t pairs, const float *ref_logp, const float *w, double beta, double smooth, int32_t mean,
+                                     float *loss, float *margin, float *logp, void *grad, int64_t ldg, void *work);
 
 #ifdef __cplusplus
 }
