@@ -79,169 +79,589 @@ __device__ __forceinline__ RowLoss policy_row(float lp, float old_lp, float adv,
     return o;
 }
 
-// What the threads of a CTA find, joined in a fixed order: every thread gets it.  s_red: 33 floats
-template <typename F>
-__device__ __forceinline__ float block_all(float v, F f, float *s_red) {
-    for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(FULL, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = s_red[0];
-    for (int q = 1; q < (int)(blockDim.x >> 5); ++q) v = f(v, s_red[q]);
+// ---------------------------------------------------------------------------------- rows in registers
+// A row is cut into granules of 16 bytes, as memory is, not as the row begins: element k sits in granule (k + off) / E, off = elements of the
+// first granule that come before the row.  Elements outside of the row read as -inf and are not written.
+template <typename ZT> struct Pack;
+template <> struct Pack<float> {
+    static constexpr int E = 4;
+    static constexpr uint32_t NONE = 0xff800000u;
+    static __device__ __forceinline__ void get(const uint4 &r, float (&x)[4]) {
+        x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
+    }
+    static __device__ __forceinline__ uint4 put(const float (&x)[4]) {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    }
+    static __device__ __forceinline__ float largest(const uint4 &r) {
+        return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+    }
+};
+template <> struct Pack<__nv_bfloat16> {
+    static constexpr int E = 8;
+    static constexpr uint32_t NONE = 0xff80ff80u;
+    static __device__ __forceinline__ void two(uint32_t w, float &a, float &b) { a = __uint_as_float(w << 16); b = __uint_as_float(w & 0xffff0000u); }
+    static __device__ __forceinline__ void get(const uint4 &r, float (&x)[8]) {
+        two(r.x, x[0], x[1]); two(r.y, x[2], x[3]); two(r.z, x[4], x[5]); two(r.w, x[6], x[7]);
+    }
+    static __device__ __forceinline__ uint32_t join2(float a, float b) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+    static __device__ __forceinline__ uint4 put(const float (&x)[8]) { return make_uint4(join2(x[0], x[1]), join2(x[2], x[3]), join2(x[4], x[5]), join2(x[6], x[7])); }
+    static __device__ __forceinline__ float largest(const uint4 &r) {
+        const __nv_bfloat162 *v = reinterpret_cast<const __nv_bfloat162 *>(&r);
+        const float2 f = __bfloat1622float2(__hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
+        return fmaxf(f.x, f.y);
+    }
+};
+template <> struct Pack<__half> {
+    static constexpr int E = 8;
+    static constexpr uint32_t NONE = 0xfc00fc00u;
+    static __device__ __forceinline__ void two(uint32_t w, float &a, float &b) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+        a = f.x; b = f.y;
+    }
+    static __device__ __forceinline__ void get(const uint4 &r, float (&x)[8]) {
+        two(r.x, x[0], x[1]); two(r.y, x[2], x[3]); two(r.z, x[4], x[5]); two(r.w, x[6], x[7]);
+    }
+    static __device__ __forceinline__ uint32_t join2(float a, float b) {
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+    static __device__ __forceinline__ uint4 put(const float (&x)[8]) { return make_uint4(join2(x[0], x[1]), join2(x[2], x[3]), join2(x[4], x[5]), join2(x[6], x[7])); }
+    static __device__ __forceinline__ float largest(const uint4 &r) {
+        const __half2 *v = reinterpret_cast<const __half2 *>(&r);
+        const float2 f = __half22float2(__hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
+        return fmaxf(f.x, f.y);
+    }
+};
+
+// Where a row lies
+template <typename ZT> struct RowAt {
+    static constexpr int E = Pack<ZT>::E;
+    const ZT *z;
+    ZT *g, *h;
+    const char *lo, *hi;    // the array's ends
+    int K, off, nvec;
+    bool gv, hv;            // whole granules of g, h can be written: they begin where those of z do
+    __device__ __forceinline__ RowAt(const SoftArgs &a, long long row) {
+        z = static_cast<const ZT *>(a.z) + row * a.ldz;
+        g = a.g ? static_cast<ZT *>(a.g) + row * a.ldg : nullptr;
+        h = a.h ? static_cast<ZT *>(a.h) + row * a.ldh : nullptr;
+        lo = static_cast<const char *>(a.z);
+        hi = reinterpret_cast<const char *>(static_cast<const ZT *>(a.z) + (a.n - 1) * a.ldz + a.K);
+        K = a.K;
+        off = (int)((uintptr_t)z & 15) / (int)sizeof(ZT);
+        nvec = (K + off + E - 1) / E;
+        gv = ((((uintptr_t)g) ^ (uintptr_t)z) & 15) == 0;
+        hv = ((((uintptr_t)h) ^ (uintptr_t)z) & 15) == 0;
+    }
+    __device__ __forceinline__ bool inside(int v) const { return v * E >= off && v * E - off + E <= K; }
+    __device__ __forceinline__ uint4 load(int v) const {
+        const char *p = reinterpret_cast<const char *>(z - off) + (size_t)v * 16;
+        if (inside(v)) return fetch(p);
+        // the ends of a row: a granule that belongs to the array is read whole, else element by element
+        uint4 r = make_uint4(Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE);
+        ZT *x = reinterpret_cast<ZT *>(&r);
+        if (p >= lo && p + 16 <= hi) {
+            const uint4 q = fetch(p);
+            const ZT *y = reinterpret_cast<const ZT *>(&q);
+#pragma unroll
+            for (int e = 0; e < E; ++e) if ((unsigned)(v * E - off + e) < (unsigned)K) x[e] = y[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) if ((unsigned)(v * E - off + e) < (unsigned)K) x[e] = z[v * E - off + e];
+        }
+        return r;
+    }
+    static __device__ __forceinline__ uint4 fetch(const char *p) { return __ldg(reinterpret_cast<const uint4 *>(p)); }
+    __device__ __forceinline__ void store(ZT *o, bool whole, int v, const float (&x)[E]) const {
+        if (whole && inside(v)) { *reinterpret_cast<uint4 *>(o + (v * E - off)) = Pack<ZT>::put(x); return; }
+#pragma unroll
+        for (int e = 0; e < E; ++e) if ((unsigned)(v * E - off + e) < (unsigned)K) o[v * E - off + e] = from_f<ZT>(x[e]);
+    }
+    __device__ __forceinline__ void fill(int v, float value) const {
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = value;
+        if (g) store(g, gv, v, x);
+        if (h) store(h, hv, v, x);
+    }
+};
+
+__device__ __forceinline__ float ex2(float x) { // of results below 2^-126 nothing is left
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// joined by `width` lanes that lie side by side, in a fixed order; every one of them gets it
+__device__ __forceinline__ float lanes_sum(float v, int width) {
+    for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
     return v;
 }
-__device__ __forceinline__ float sum2(float a, float b) { return a + b; }
+__device__ __forceinline__ float lanes_max(float v, int width) {
+    for (int o = width >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+    return v;
+}
+__device__ __forceinline__ Soft lanes_join(Soft r, float c, int width) {
+    const float m = lanes_max(r.m, width);
+    return {m, lanes_sum(r.s * ex2((r.m - base_of(m)) * c), width)};
+}
 
-// One CTA walks over a row twice: maximum and sum, then gradient.
-template <typename ZT, int KIND>
-__global__ void __launch_bounds__(256) k_rows(SoftArgs a) {
-    extern __shared__ __align__(16) unsigned char s_raw[];
-    __shared__ float s_red[33];
-    const int K = a.K, tid = threadIdx.x, nt = blockDim.x;
+// Maximum and sum of a thread's V granules; `bits(i)`: elements of granule i to leave out.  32-bit elements become their terms (relative to the
+// thread's maximum), so that no exponential is worked out twice; 16-bit ones stay: their terms would take twice the registers.
+template <typename ZT, int V, typename F>
+__device__ __forceinline__ Soft take(uint4 (&r)[V], float c, bool exclude, F bits) {
+    constexpr int E = Pack<ZT>::E;
+    if (exclude) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const unsigned b = bits(i);
+            if (b) {
+                ZT *x = reinterpret_cast<ZT *>(&r[i]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) if (b >> e & 1u) x[e] = from_f<ZT>(-INFINITY);
+            }
+        }
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; ++i) m = fmaxf(m, Pack<ZT>::largest(r[i]));
+    const float base = base_of(m);
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        float x[E];
+        Pack<ZT>::get(r[i], x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) { x[e] = ex2((x[e] - base) * c); s[e & 1] += x[e]; }
+        if (E == 4) r[i] = Pack<ZT>::put(x);
+        else asm volatile("" : "+r"(r[i].x), "+r"(r[i].y), "+r"(r[i].z), "+r"(r[i].w)); // they stay packed: unpacked they would take twice the registers
+    }
+    return {m, s[0] + s[1]};
+}
+
+// Slots of a row in shared memory
+struct Slots {
+    int *id;            // class, 0-based, -1: none
+    float *t, *z;       // what the teacher has, the row's prediction
+    float *q, *lp;      // probability, log p: written by slots_row
+    static constexpr int BYTES = 20;
+    __device__ __forceinline__ Slots(void *p, int T) {
+        id = static_cast<int *>(p);
+        t = reinterpret_cast<float *>(id + T);
+        z = t + T; q = z + T; lp = q + T;
+    }
+};
+struct RowOut {
+    float m, A, B;      // gradient A e and probability B e of the classes that are not named, e = 2^(c (z - m))
+    float mass;         // distillation: sum of the teacher's probabilities; else: factor of (delta - p)
+    float hw;           // hessian hw p (1 - p)
+    float lp;           // log p of the class taken
+    float loss;
+};
+__device__ __forceinline__ bool first_slot(const Slots &s, int j) {
+    for (int i = 0; i < j; ++i) if (s.id[i] == s.id[j]) return false;
+    return true;
+}
+// r: what the scan found.  `width` lanes share the slots; `keep`: these lanes write q and lp
+__device__ __forceinline__ RowOut slots_row(const SoftArgs &a, const Slots &s, Soft r, bool dup, float w, int lane, int width, bool keep) {
     const float c = a.c;
-    // distillation: class (0-based, -1: none), probability, prediction of every slot; then a bit for every class that is named
-    int *s_id = reinterpret_cast<int *>(s_raw);
-    float *s_q = reinterpret_cast<float *>(s_id + a.T), *s_z = s_q + a.T;
-    uint32_t *s_bits = reinterpret_cast<uint32_t *>(s_z + a.T);
-    for (long long row = blockIdx.x; row < a.n; row += gridDim.x) {
-        const ZT *z = static_cast<const ZT *>(a.z) + row * a.ldz;
-        ZT *g = a.g ? static_cast<ZT *>(a.g) + row * a.ldg : nullptr, *h = a.h ? static_cast<ZT *>(a.h) + row * a.ldh : nullptr;
-        float w = a.w ? a.w[row * a.w_stride] : 1.0f;
-        bool live = w != 0.0f, bad = false;
-        int code = -1;
+    float tmax = -INFINITY, zmax = r.m;
+    for (int j = lane; j < a.T; j += width) if (s.id[j] >= 0) { tmax = fmaxf(tmax, s.t[j]); zmax = fmaxf(zmax, s.z[j]); }
+    if (!a.tail) tmax = lanes_max(tmax, width);
+    zmax = lanes_max(zmax, width);
+    const float base = base_of(zmax);
+    float Q = 0.0f, named = 0.0f;
+    for (int j = lane; j < a.T; j += width) {
+        if (s.id[j] < 0) continue;
+        Q += a.tail ? expf(s.t[j]) : expf((s.t[j] - tmax) * a.inv_tau);
+        if (a.tail && (!dup || first_slot(s, j))) named += ex2((s.z[j] - base) * c);
+    }
+    Q = lanes_sum(Q, width);
+    Soft all = r;
+    if (a.tail) all = {zmax, lanes_sum(named, width) + r.s * ex2((r.m - base) * c)};
+    const float ls = logf(all.s), lq = logf(Q);
+    float loss = 0.0f;
+    for (int j = lane; j < a.T; j += width) {
+        if (s.id[j] < 0) continue;
+        const float lt = a.tail ? s.t[j] : (s.t[j] - tmax) * a.inv_tau - lq, q = expf(lt), lp = (s.z[j] - all.m) * a.inv_tau - ls;
+        if (keep) { s.q[j] = q; s.lp[j] = lp; }
+        if (q != 0.0f) loss += q * (lt - lp);
+    }
+    loss = lanes_sum(loss, width);
+    // the rest, when there is any: no class is left where every one is named or ruled out
+    const float qt = a.tail && r.m != -INFINITY ? fmaxf(0.0f, 1.0f - Q) : 0.0f;
+    if (qt > 0.0f) loss += qt * (logf(qt) - ((r.m - all.m) * a.inv_tau + logf(r.s) - ls));
+    RowOut o;
+    o.m = base_of(r.m);
+    o.mass = a.tail ? Q + qt : 1.0f;
+    o.B = r.m == -INFINITY ? 0.0f * ls : ex2((r.m - base_of(all.m)) * c) / all.s;
+    o.A = w * a.tau * (o.mass * o.B - (qt > 0.0f ? qt / r.s : 0.0f));
+    o.hw = w;
+    o.loss = w * a.tau * a.tau * loss;
+    return o;
+}
+template <int KIND>
+__device__ __forceinline__ RowOut class_row(const SoftArgs &a, Soft r, float za, long long row, float w) {
+    RowOut o;
+    o.m = base_of(r.m);
+    o.B = 1.0f / r.s;
+    o.lp = (za - r.m) * a.inv_tau - logf(r.s);
+    o.mass = 0.0f;
+    o.loss = 0.0f;
+    if (KIND == ROW_POLICY) {
+        const long long i = row * a.p_stride;
+        const RowLoss l = policy_row(o.lp, a.old_lp[i], a.adv[i], a.ref, i, a.lo, a.hi, a.beta);
+        o.loss = w * l.loss;
+        o.mass = w * l.d * a.inv_tau;
+    }
+    o.A = -o.mass * o.B;
+    o.hw = w * a.inv_tau * a.inv_tau;
+    return o;
+}
+// The gradient (and hessian) of a thread's granule v: `x` holds its elements' terms
+template <typename ZT, int KIND, int E>
+__device__ __forceinline__ void put_terms(const SoftArgs &a, const RowAt<ZT> &at, const RowOut &o, int v, const float (&x)[E], float scale, int code) {
+    float y[E];
+    if (at.g) {
+        const float A = o.A * scale;
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = x[e] * A;
+        if (KIND != ROW_DISTILL && v == (code + at.off) / E) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) if (v * E + e == code + at.off) y[e] = -o.mass * expm1f(o.lp); // 1 - p, also where p is close to 1
+        }
+        at.store(at.g, at.gv, v, y);
+    }
+    if (at.h) {
+        const float B = o.B * scale;
+#pragma unroll
+        for (int e = 0; e < E; ++e) { const float p = x[e] * B; y[e] = o.hw * p * (1.0f - p); }
+        at.store(at.h, at.hv, v, y);
+    }
+}
+// the named classes, after all others have been written
+template <typename ZT>
+__device__ __forceinline__ void put_slot(const SoftArgs &a, const RowAt<ZT> &at, const RowOut &o, const Slots &s, int j, bool dup, float w) {
+    float q = s.q[j];
+    if (dup) {
+        if (!first_slot(s, j)) return;
+        q = 0.0f;
+        for (int i = j; i < a.T; ++i) if (s.id[i] == s.id[j]) q += s.q[i];
+    }
+    const float p = expf(s.lp[j]);
+    if (at.g) at.g[s.id[j]] = from_f<ZT>(w * a.tau * (o.mass * p - q));
+    if (at.h) at.h[s.id[j]] = from_f<ZT>(o.hw * p * (1.0f - p));
+}
+
+enum { SLOT_SOME = 1, SLOT_BAD = 2, SLOT_TWICE = 4 };
+// Slot j of a row into shared memory; the classes named in granules v0 .. v1 - 1 are marked in `bits` (bit: element from the first of granule v0)
+template <typename ZT>
+__device__ __forceinline__ int put_into(const SoftArgs &a, const RowAt<ZT> &at, const Slots &s, uint32_t *bits, long long row, int j, int v0, int v1) {
+    const uint32_t id = a.ids[row * a.ldt + j];
+    const float t = load_t(a.t, a.t_dtype, row * a.ldt + j);
+    const bool use = id != 0u && t != -INFINITY, ok = use && id <= (uint32_t)a.K;
+    s.id[j] = ok ? (int)id - 1 : -1;
+    s.t[j] = t;
+    s.z[j] = ok ? to_f(at.z[id - 1]) : 0.0f;
+    int flags = (use ? SLOT_SOME : 0) | (use && !ok ? SLOT_BAD : 0);
+    const int b = (int)id - 1 + at.off - v0 * RowAt<ZT>::E;
+    if (ok && b >= 0 && b < (v1 - v0) * RowAt<ZT>::E && (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u)) flags |= SLOT_TWICE;
+    return flags;
+}
+template <int E> __device__ __forceinline__ unsigned granule_bits(const uint32_t *bits, int u) { return bits[u * E >> 5] >> (u * E & 31) & ((1u << E) - 1u); }
+
+// Rows of up to V granules for each of G lanes (a power of two up to 32): 32 / G rows a warp, 8 warps a CTA.
+template <typename ZT, int KIND, int V>
+__global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words) {
+    extern __shared__ __align__(16) unsigned char s_raw[];
+    constexpr int E = Pack<ZT>::E;
+    const int lane = threadIdx.x & (G - 1), group = threadIdx.x / G;
+    const long long row0 = (long long)blockIdx.x * (256 / G) + group;
+    const bool there = row0 < a.n;
+    const long long row = there ? row0 : a.n - 1;
+    const RowAt<ZT> at(a, row);
+    unsigned char *mine = s_raw + (size_t)group * (KIND == ROW_DISTILL ? a.T * Slots::BYTES + words * 4 : 0);
+    const Slots s(mine, KIND == ROW_DISTILL ? a.T : 0);
+    uint32_t *bits = reinterpret_cast<uint32_t *>(mine + (size_t)a.T * Slots::BYTES);
+    float w = a.w ? a.w[row * a.w_stride] : 1.0f;
+    if (KIND == ROW_COEF) w = a.coef[row];
+    uint32_t id = 0u;
+    if (KIND != ROW_DISTILL) id = a.code[row * a.p_stride];
+    bool live = there && w != 0.0f && (KIND == ROW_DISTILL || id != 0u);
+    int flags = 0;
+    uint4 r[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int v = lane + i * G;
+        r[i] = live && v < at.nvec ? at.load(v) : make_uint4(Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE);
+    }
+    if (KIND == ROW_DISTILL) {
+        for (int i = lane; i < words; i += G) bits[i] = 0u;
+        __syncwarp();
+        if (live) for (int j = lane; j < a.T; j += G) flags |= put_into(a, at, s, bits, row, j, 0, at.nvec);
+        for (int o = G >> 1; o > 0; o >>= 1) flags |= __shfl_xor_sync(FULL, flags, o);
+        __syncwarp();
+        live = live && (flags & SLOT_SOME);
+    } else if (live && id > (uint32_t)a.K) flags = SLOT_BAD;
+    const bool whole = live && !(flags & SLOT_BAD);
+    const int code = whole && KIND != ROW_DISTILL ? (int)id - 1 : -1;
+    const float za = code >= 0 ? to_f(at.z[code]) : 0.0f;
+    if (there && !whole) {
+        const float value = live ? NAN : 0.0f;
+        if (KIND != ROW_LOGP) for (int v = lane; v < at.nvec; v += G) at.fill(v, value);
+        if (lane == 0) {
+            if (KIND != ROW_COEF && a.loss) a.loss[row] = value;
+            if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = value;
+            if (KIND == ROW_LOGP) a.stat[row] = make_float2(0.0f, value);
+        }
+    }
+    Soft mine_r = {0.0f, 1.0f}, all = mine_r;
+    RowOut o = {};
+    if (KIND == ROW_COEF) {
+        if (whole) {
+            const float2 st = a.stat[row];
+            o.m = base_of(st.x); o.B = st.y; o.lp = a.logp[row]; o.mass = w; o.A = -w * st.y;
+        }
+    } else {
+        mine_r = take<ZT, V>(r, a.c, KIND == ROW_DISTILL && a.tail && whole, [&](int i) {
+            const int v = lane + i * G;
+            return v < at.nvec ? granule_bits<E>(bits, v) : 0u; });
+        all = lanes_join(mine_r, a.c, G);
+        if (KIND == ROW_DISTILL) { if (!whole) for (int j = lane; j < a.T; j += G) s.id[j] = -1; __syncwarp(); o = slots_row(a, s, all, flags & SLOT_TWICE, w, lane, G, true); }
+        else if (whole) o = class_row<KIND>(a, all, za, row, w);
+    }
+    if (whole) {
+        if (lane == 0) {
+            if ((KIND == ROW_DISTILL || KIND == ROW_POLICY) && a.loss) a.loss[row] = o.loss;
+            if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = o.lp;
+            if (KIND == ROW_LOGP) a.stat[row] = make_float2(all.m, o.B);
+        }
+        const float scale = E == 4 && KIND != ROW_COEF ? ex2((mine_r.m - o.m) * a.c) : 1.0f;
+        if (KIND != ROW_LOGP && (at.g || at.h)) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int v = lane + i * G;
+                if (v < at.nvec) {
+                    float x[E];
+                    Pack<ZT>::get(r[i], x);
+                    if (E == 8 || KIND == ROW_COEF) {
+#pragma unroll
+                        for (int e = 0; e < E; ++e) x[e] = ex2((x[e] - o.m) * a.c);
+                    }
+                    put_terms<ZT, KIND>(a, at, o, v, x, scale, code);
+                }
+            }
+        }
+    }
+    if (KIND == ROW_DISTILL) {
+        __syncwarp();
+        if (whole && (at.g || at.h)) for (int j = lane; j < a.T; j += G) if (s.id[j] >= 0) put_slot(a, at, o, s, j, flags & SLOT_TWICE, w);
+    }
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float2 cluster_read(const float2 *p, int rank) {
+    uint32_t at;
+    float2 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ int cluster_read(const int *p, int rank) {
+    uint32_t at;
+    int v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// One row for a CTA, or for a cluster of CS CTAs, up to V granules a thread.
+template <typename ZT, int KIND, int V>
+__global__ void __launch_bounds__(V > 4 ? 512 : 1024) k_row_ctas(SoftArgs a, int CS, int words) {
+    extern __shared__ __align__(16) unsigned char s_raw[];
+    __shared__ float2 s_part[32];
+    __shared__ float2 s_cta;
+    __shared__ int s_flags;
+    constexpr int E = Pack<ZT>::E;
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warps = nt >> 5;
+    const long long row = blockIdx.x / (unsigned)CS;
+    const int rank = CS > 1 ? (int)(blockIdx.x % (unsigned)CS) : 0;
+    const RowAt<ZT> at(a, row);
+    const int per = (at.nvec + CS - 1) / CS, v0 = min(rank * per, at.nvec), v1 = min(v0 + per, at.nvec);
+    const Slots s(s_raw, KIND == ROW_DISTILL ? a.T : 0);
+    uint32_t *bits = reinterpret_cast<uint32_t *>(s_raw + (size_t)a.T * Slots::BYTES);
+    float w = a.w ? a.w[row * a.w_stride] : 1.0f;
+    if (KIND == ROW_COEF) w = a.coef[row];
+    uint32_t id = 0u;
+    if (KIND != ROW_DISTILL) id = a.code[row * a.p_stride];
+    bool live = w != 0.0f && (KIND == ROW_DISTILL || id != 0u);
+    uint4 r[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int v = v0 + tid + i * nt;
+        r[i] = live && v < v1 ? at.load(v) : make_uint4(Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE);
+    }
+    int flags = live && KIND != ROW_DISTILL && id > (uint32_t)a.K ? SLOT_BAD : 0;
+    if (KIND == ROW_DISTILL && live) {
+        if (tid == 0) s_flags = 0;
+        for (int i = tid; i < words; i += nt) bits[i] = 0u;
+        __syncthreads();
+        for (int j = tid; j < a.T; j += nt) flags |= put_into(a, at, s, bits, row, j, v0, v1);
+        flags = __reduce_or_sync(FULL, flags);
+        if (lane == 0 && flags) atomicOr(&s_flags, flags);
+        __syncthreads();
+        flags = s_flags;
+        live = flags & SLOT_SOME;
+    }
+    if (!live || (flags & SLOT_BAD)) {
+        const float value = live ? NAN : 0.0f;
+        if (KIND != ROW_LOGP) for (int v = v0 + tid; v < v1; v += nt) at.fill(v, value);
+        if (tid == 0 && rank == 0) {
+            if (KIND != ROW_COEF && a.loss) a.loss[row] = value;
+            if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = value;
+            if (KIND == ROW_LOGP) a.stat[row] = make_float2(0.0f, value);
+        }
+        return;
+    }
+    const int code = KIND != ROW_DISTILL ? (int)id - 1 : -1;
+    const float za = code >= 0 ? to_f(at.z[code]) : 0.0f;
+    Soft mine = {0.0f, 1.0f}, all = mine;
+    RowOut o = {};
+    if (KIND == ROW_COEF) {
+        const float2 st = a.stat[row];
+        o.m = base_of(st.x); o.B = st.y; o.lp = a.logp[row]; o.mass = w; o.A = -w * st.y;
+    } else {
+        mine = take<ZT, V>(r, a.c, KIND == ROW_DISTILL && a.tail, [&](int i) {
+            const int v = v0 + tid + i * nt;
+            return v < v1 ? granule_bits<E>(bits, v - v0) : 0u; });
+        all = lanes_join(mine, a.c, 32);
+        if (lane == 0) s_part[tid >> 5] = make_float2(all.m, all.s);
+        __syncthreads();
+        const float2 p = lane < warps ? s_part[lane] : make_float2(-INFINITY, 0.0f);
+        all = lanes_join(Soft{p.x, p.y}, a.c, 32);
+        if (CS > 1) {
+            if (tid == 0) s_cta = make_float2(all.m, all.s);
+            cluster_arrive();
+            cluster_wait();
+            const float2 q = lane < CS ? cluster_read(&s_cta, lane) : make_float2(-INFINITY, 0.0f);
+            all = lanes_join(Soft{q.x, q.y}, a.c, 32);
+            if (KIND == ROW_DISTILL) flags |= __reduce_or_sync(FULL, lane < CS ? cluster_read(&s_flags, lane) : 0); // each sees its own classes twice
+            cluster_arrive(); // a CTA that has read may let the others go: they wait for it at their end
+        }
+        if (KIND == ROW_DISTILL) o = slots_row(a, s, all, flags & SLOT_TWICE, w, lane, 32, tid < 32);
+        else o = class_row<KIND>(a, all, za, row, w);
+    }
+    if (tid == 0 && rank == 0) {
+        if ((KIND == ROW_DISTILL || KIND == ROW_POLICY) && a.loss) a.loss[row] = o.loss;
+        if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = o.lp;
+        if (KIND == ROW_LOGP) a.stat[row] = make_float2(all.m, o.B);
+    }
+    if (KIND != ROW_LOGP && (at.g || at.h)) {
+        const float scale = E == 4 && KIND != ROW_COEF ? ex2((mine.m - o.m) * a.c) : 1.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int v = v0 + tid + i * nt;
+            if (v < v1) {
+                float x[E];
+                Pack<ZT>::get(r[i], x);
+                if (E == 8 || KIND == ROW_COEF) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x[e] = ex2((x[e] - o.m) * a.c);
+                }
+                put_terms<ZT, KIND>(a, at, o, v, x, scale, code);
+            }
+        }
         if (KIND == ROW_DISTILL) {
-            bool some = false;
-            __syncthreads();
-            if (a.tail) for (int i = tid; i < (K + 31) / 32; i += nt) s_bits[i] = 0u;
-            __syncthreads();
-            for (int j = tid; j < a.T && live; j += nt) {
-                const uint32_t id = a.ids[row * a.ldt + j];
-                const float t = load_t(a.t, a.t_dtype, row * a.ldt + j);
-                const bool use = id != 0u && t != -INFINITY, ok = id <= (uint32_t)K;
-                some |= use; bad |= use && !ok;
-                s_id[j] = use && ok ? (int)id - 1 : -1;
-                s_q[j] = t;
-                s_z[j] = use && ok ? to_f(z[id - 1]) : 0.0f;
-                if (a.tail && use && ok) atomicOr(&s_bits[(id - 1) >> 5], 1u << ((id - 1) & 31));
-            }
-            live = __syncthreads_or(live && some);
-            bad = __syncthreads_or(bad);
-        } else {
-            const uint32_t id = a.code[row * a.p_stride];
-            if (KIND == ROW_COEF) w = a.coef[row];
-            live = live && id != 0u && w != 0.0f;
-            bad = live && id > (uint32_t)K;
-            if (live && !bad) code = (int)id - 1;
-        }
-        if (!live || bad) { // a row that does not count; a class that there is not: NaN
-            const float v = bad ? NAN : 0.0f;
-            for (int k = tid; k < K; k += nt) { if (g) g[k] = from_f<ZT>(v); if (h) h[k] = from_f<ZT>(v); }
-            if (tid == 0) {
-                if (a.loss) a.loss[row] = v;
-                if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = v;
-                if (KIND == ROW_LOGP) a.stat[row] = make_float2(0.0f, v);
-            }
-            continue;
-        }
-        Soft r = {-INFINITY, 0.0f};
-        if (KIND != ROW_COEF) {
-            const bool tail = KIND == ROW_DISTILL && a.tail;
-            for (int k = tid; k < K; k += nt) {
-                if (tail && (s_bits[k >> 5] >> (k & 31) & 1u)) continue;
-                r = join(r, Soft{to_f(z[k]), 1.0f}, c);
-            }
-            const float m = block_all(r.m, [](float x, float y) { return fmaxf(x, y); }, s_red), base = base_of(m);
-            r.s = block_all(r.s * term(r.m, base, c), sum2, s_red);
-            r.m = m;
-        }
-        float A, B; // g = A e, p = B e with e = 2^(c (z - max))
-        if (KIND == ROW_DISTILL) {
-            float tmax = -INFINITY, zmax = r.m, Q = 0.0f;
-            for (int j = tid; j < a.T; j += nt) if (s_id[j] >= 0) { tmax = fmaxf(tmax, s_q[j]); zmax = fmaxf(zmax, s_z[j]); }
-            tmax = block_all(tmax, [](float x, float y) { return fmaxf(x, y); }, s_red);
-            zmax = block_all(zmax, [](float x, float y) { return fmaxf(x, y); }, s_red);
-            // named classes, each of them once
-            const float base = base_of(zmax);
-            float s = 0.0f;
-            for (int j = tid; j < a.T; j += nt) {
-                if (s_id[j] < 0) continue;
-                Q += a.tail ? expf(s_q[j]) : expf((s_q[j] - tmax) * a.inv_tau);
-                bool first = true;
-                for (int i = 0; i < j; ++i) first = first && s_id[i] != s_id[j];
-                if (first) s += term(s_z[j], base, c);
-            }
-            Q = block_all(Q, sum2, s_red);
-            s = block_all(s, sum2, s_red);
-            const Soft all = a.tail ? Soft{zmax, s + r.s * term(r.m, base, c)} : r;
-            const float ls = logf(all.s), lq = logf(Q);
-            float loss = 0.0f;
             __syncthreads();
             for (int j = tid; j < a.T; j += nt) {
-                if (s_id[j] < 0) continue;
-                const float lt = a.tail ? s_q[j] : (s_q[j] - tmax) * a.inv_tau - lq, q = expf(lt);
-                const float lp = (s_z[j] - all.m) * a.inv_tau - ls;
-                s_q[j] = q;
-                s_z[j] = lp;
-                if (q != 0.0f) loss += q * (lt - lp);
-            }
-            float qt = 0.0f;
-            if (a.tail && r.m != -INFINITY) qt = fmaxf(0.0f, 1.0f - Q);
-            const float mass = a.tail ? Q + qt : 1.0f;
-            loss = block_all(loss, sum2, s_red);
-            if (qt > 0.0f) loss += qt * (logf(qt) - ((r.m - all.m) * a.inv_tau + logf(r.s) - ls));
-            if (tid == 0 && a.loss) a.loss[row] = w * a.tau * a.tau * loss;
-            B = r.m == -INFINITY ? 0.0f * ls : term(r.m, base_of(all.m), c) / all.s;
-            A = w * a.tau * (mass * B - (qt > 0.0f ? qt / r.s : 0.0f));
-            const float m1 = base_of(r.m);
-            for (int k = tid; k < K && (g || h); k += nt) {
-                const float e = term(to_f(z[k]), m1, c), p = e * B;
-                if (g) g[k] = from_f<ZT>(e * A);
-                if (h) h[k] = from_f<ZT>(w * p * (1.0f - p));
-            }
-            __syncthreads();
-            for (int j = tid; j < a.T && (g || h); j += nt) {
-                if (s_id[j] < 0) continue;
-                bool first = true;
-                for (int i = 0; i < j; ++i) first = first && s_id[i] != s_id[j];
-                if (!first) continue;
-                float q = 0.0f;
-                for (int i = j; i < a.T; ++i) if (s_id[i] == s_id[j]) q += s_q[i];
-                const float p = expf(s_z[j]);
-                if (g) g[s_id[j]] = from_f<ZT>(w * a.tau * (mass * p - q));
-                if (h) h[s_id[j]] = from_f<ZT>(w * p * (1.0f - p));
-            }
-        } else {
-            const float za = to_f(z[code]);
-            float lp, f; // f: factor of (delta - p)
-            if (KIND == ROW_COEF) {
-                const float2 st = a.stat[row];
-                r.m = st.x;
-                B = st.y;
-                lp = a.logp[row];
-                f = w;
-            } else {
-                lp = (za - r.m) * a.inv_tau - logf(r.s);
-                B = 1.0f / r.s;
-                f = 0.0f;
-            }
-            if (KIND == ROW_LOGP) {
-                if (tid == 0) { a.logp[row] = lp; a.stat[row] = make_float2(r.m, B); }
-                continue;
-            }
-            if (KIND == ROW_POLICY) {
-                const long long i = row * a.p_stride;
-                const RowLoss o = policy_row(lp, a.old_lp[i], a.adv[i], a.ref, i, a.lo, a.hi, a.beta);
-                if (tid == 0) { if (a.loss) a.loss[row] = w * o.loss; if (a.logp) a.logp[row] = lp; }
-                f = w * o.d * a.inv_tau;
-            }
-            A = -f * B;
-            const float m1 = base_of(r.m), hw = w * a.inv_tau * a.inv_tau;
-            for (int k = tid; k < K && (g || h); k += nt) {
-                const float e = term(to_f(z[k]), m1, c), p = e * B;
-                if (g) g[k] = k == code ? from_f<ZT>(-f * expm1f(lp)) : from_f<ZT>(e * A);
-                if (h) h[k] = from_f<ZT>(hw * p * (1.0f - p));
+                const int k = s.id[j], v = (k + at.off) / E;
+                if (k >= 0 && v >= v0 && v < v1) put_slot(a, at, o, s, j, flags & SLOT_TWICE, w);
             }
         }
+    }
+    if (CS > 1 && KIND != ROW_COEF) cluster_wait();
+}
+
+// Rows of more granules than a cluster holds: one CTA walks over a row twice.
+template <typename ZT, int KIND>
+__global__ void __launch_bounds__(512) k_row_walk(SoftArgs a, int words) {
+    extern __shared__ __align__(16) unsigned char s_raw[];
+    __shared__ float2 s_part[32];
+    __shared__ int s_flags;
+    constexpr int E = Pack<ZT>::E;
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warps = nt >> 5;
+    const long long row = blockIdx.x;
+    const RowAt<ZT> at(a, row);
+    const Slots s(s_raw, KIND == ROW_DISTILL ? a.T : 0);
+    uint32_t *bits = reinterpret_cast<uint32_t *>(s_raw + (size_t)a.T * Slots::BYTES);
+    float w = a.w ? a.w[row * a.w_stride] : 1.0f;
+    if (KIND == ROW_COEF) w = a.coef[row];
+    uint32_t id = 0u;
+    if (KIND != ROW_DISTILL) id = a.code[row * a.p_stride];
+    bool live = w != 0.0f && (KIND == ROW_DISTILL || id != 0u);
+    int flags = live && KIND != ROW_DISTILL && id > (uint32_t)a.K ? SLOT_BAD : 0;
+    if (KIND == ROW_DISTILL && live) {
+        if (tid == 0) s_flags = 0;
+        for (int i = tid; i < words; i += nt) bits[i] = 0u;
+        __syncthreads();
+        for (int j = tid; j < a.T; j += nt) flags |= put_into(a, at, s, bits, row, j, 0, at.nvec);
+        flags = __reduce_or_sync(FULL, flags);
+        if (lane == 0 && flags) atomicOr(&s_flags, flags);
+        __syncthreads();
+        flags = s_flags;
+        live = flags & SLOT_SOME;
+    }
+    if (!live || (flags & SLOT_BAD)) {
+        const float value = live ? NAN : 0.0f;
+        if (KIND != ROW_LOGP) for (int v = tid; v < at.nvec; v += nt) at.fill(v, value);
+        if (tid == 0) {
+            if (KIND != ROW_COEF && a.loss) a.loss[row] = value;
+            if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = value;
+            if (KIND == ROW_LOGP) a.stat[row] = make_float2(0.0f, value);
+        }
+        return;
+    }
+    const int code = KIND != ROW_DISTILL ? (int)id - 1 : -1;
+    const float za = code >= 0 ? to_f(at.z[code]) : 0.0f;
+    RowOut o = {};
+    if (KIND == ROW_COEF) {
+        const float2 st = a.stat[row];
+        o.m = base_of(st.x); o.B = st.y; o.lp = a.logp[row]; o.mass = w; o.A = -w * st.y;
+    } else {
+        Soft all = {-INFINITY, 0.0f};
+        for (int v = tid; v < at.nvec; v += nt) {
+            uint4 r[1] = {at.load(v)};
+            all = join(all, take<ZT, 1>(r, a.c, KIND == ROW_DISTILL && a.tail, [&](int) { return granule_bits<E>(bits, v); }), a.c);
+        }
+        all = lanes_join(all, a.c, 32);
+        if (lane == 0) s_part[tid >> 5] = make_float2(all.m, all.s);
+        __syncthreads();
+        const float2 p = lane < warps ? s_part[lane] : make_float2(-INFINITY, 0.0f);
+        all = lanes_join(Soft{p.x, p.y}, a.c, 32);
+        if (KIND == ROW_DISTILL) o = slots_row(a, s, all, flags & SLOT_TWICE, w, lane, 32, tid < 32);
+        else o = class_row<KIND>(a, all, za, row, w);
+        if (KIND == ROW_LOGP && tid == 0) a.stat[row] = make_float2(all.m, o.B);
+    }
+    if (tid == 0) {
+        if ((KIND == ROW_DISTILL || KIND == ROW_POLICY) && a.loss) a.loss[row] = o.loss;
+        if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = o.lp;
+    }
+    if (KIND == ROW_LOGP || !(at.g || at.h)) return;
+    for (int v = tid; v < at.nvec; v += nt) {
+        float x[E];
+        const uint4 r = at.load(v);
+        Pack<ZT>::get(r, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = ex2((x[e] - o.m) * a.c);
+        put_terms<ZT, KIND>(a, at, o, v, x, 1.0f, code);
+    }
+    if (KIND == ROW_DISTILL) {
+        __syncthreads();
+        for (int j = tid; j < a.T; j += nt) if (s.id[j] >= 0) put_slot(a, at, o, s, j, flags & SLOT_TWICE, w);
     }
 }
 
@@ -298,18 +718,70 @@ __global__ void __launch_bounds__(256) k_pairs(PairArgs a) {
     }
 }
 
+template <typename K>
+cudaError_t launch_cluster(K kern, unsigned grid, int threads, int cs, size_t smem, cudaStream_t st, const SoftArgs &a, int words) {
+    if (smem > 47 * 1024) { // with the static part
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t c = {};
+    cudaLaunchAttribute at[1];
+    c.gridDim = dim3(grid); c.blockDim = dim3(threads); c.dynamicSmemBytes = smem; c.stream = st;
+    if (cs > 1) {
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = cs; at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        c.attrs = at; c.numAttrs = 1;
+    }
+    return cudaLaunchKernelEx(&c, kern, a, cs, words);
+}
+template <typename ZT, int KIND>
+int32_t launch_typed(const SoftArgs &a, int sms, cudaStream_t st) {
+    constexpr int E = Pack<ZT>::E;
+    // granules of a row: of one that begins just before the end of its first one, unless all rows begin where a granule does
+    const bool aligned = (uintptr_t)a.z % 16 == 0 && (a.ldz % E == 0 || a.n == 1);
+    const int nvec = (a.K + (aligned ? 0 : E - 1) + E - 1) / E;
+    const size_t slots = KIND == ROW_DISTILL ? (size_t)a.T * Slots::BYTES : 0;
+    auto words_of = [&](int granules) { return KIND == ROW_DISTILL ? (granules * E + 31) / 32 : 0; };
+    if (nvec <= 256) { // within a warp
+        int G = 1, V = 1;
+        while (G < 32 && G * 8 < nvec) G *= 2;
+        while (V * G < nvec) V *= 2;
+        const int words = words_of(nvec);
+        const size_t smem = (size_t)(256 / G) * (slots + words * 4);
+        if (smem <= 200 * 1024) {
+            const unsigned grid = (unsigned)((a.n + 256 / G - 1) / (256 / G));
+            auto go = [&](void (*kern)(SoftArgs, int, int)) {
+                const cudaError_t e = smem > 47 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
+                return e != cudaSuccess ? e : evb_launch(kern, dim3(grid), dim3(256), smem, st, a, G, words);
+            };
+            EVB_CUDA(V <= 2 ? go(k_row_lanes<ZT, KIND, 2>) : V == 4 ? go(k_row_lanes<ZT, KIND, 4>) : go(k_row_lanes<ZT, KIND, 8>));
+            return EVB_OK;
+        }
+    }
+    int cs = 1;
+    while (cs < 8 && (nvec + cs - 1) / cs > 512 * 8) cs *= 2;
+    while (cs < 8 && a.n * cs * 2 <= sms && (nvec + cs - 1) / cs > 256) cs *= 2; // few rows: more SMs for each
+    const int per = (nvec + cs - 1) / cs;
+    if (per <= 512 * 8) {
+        const bool small = per <= 1024 * 2 && a.n * cs <= 2 * sms;
+        const int V = small ? 2 : 8, threads = std::max(64, ((per + V - 1) / V + 31) / 32 * 32), words = words_of(per);
+        const size_t smem = slots + words * 4;
+        EVB_CUDA(small ? launch_cluster(k_row_ctas<ZT, KIND, 2>, (unsigned)(a.n * cs), threads, cs, smem, st, a, words)
+                       : launch_cluster(k_row_ctas<ZT, KIND, 8>, (unsigned)(a.n * cs), threads, cs, smem, st, a, words));
+        return EVB_OK;
+    }
+    const int words = words_of(nvec);
+    const size_t smem = slots + words * 4;
+    if (smem > 47 * 1024) EVB_CUDA(cudaFuncSetAttribute(k_row_walk<ZT, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    EVB_CUDA(evb_launch(k_row_walk<ZT, KIND>, dim3((unsigned)a.n), dim3(512), smem, st, a, words));
+    return EVB_OK;
+}
 template <int KIND>
 int32_t launch_rows(const SoftArgs &a, int dtype, int device, cudaStream_t st) {
     int sms = 0;
     EVB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
-    const unsigned grid = (unsigned)std::min<long long>(a.n, (long long)sms * 8);
-    const size_t smem = KIND == ROW_DISTILL ? (size_t)a.T * 12 + (a.tail ? ((size_t)a.K + 31) / 32 * 4 : 0) : 0;
-    auto go = [&](void (*kern)(SoftArgs)) {
-        cudaError_t e = smem > 48 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
-        return e != cudaSuccess ? e : evb_launch(kern, dim3(grid), dim3(256), smem, st, a);
-    };
-    EVB_CUDA(dtype == EVB_BF16 ? go(k_rows<__nv_bfloat16, KIND>) : dtype == EVB_F16 ? go(k_rows<__half, KIND>) : go(k_rows<float, KIND>));
-    return EVB_OK;
+    return dtype == EVB_BF16 ? launch_typed<__nv_bfloat16, KIND>(a, sms, st) : dtype == EVB_F16 ? launch_typed<__half, KIND>(a, sms, st)
+                                                                                                : launch_typed<float, KIND>(a, sms, st);
 }
 
 // the calling thread's device is what it was when the call returns

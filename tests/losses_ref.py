@@ -145,5 +145,7 @@ def close(got, want, tol, what):
 
 def rounded(want, dtype, rel, floor):
     """Tolerance of a result that is right to `rel` of its parts (`floor`: their size) and rounded to `dtype` at the end."""
-    tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps     # half of the smallest step around zero counts too
+    # Half of the smallest step around zero counts too.  And the exponential's results below 2^-126, the smallest normal number, are zeros
+    # (the instruction flushes them): a probability is off by less than 2^-126 then, a gradient by that times its factor, at most 2^4 here.
+    tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps + 2.0 ** -122
     return rel * floor + (half_step(dtype) * (1 + rel)) * want.abs() + tiny

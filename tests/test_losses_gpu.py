@@ -11,6 +11,7 @@ NINF = float("-inf")
 DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 # around the borders of what a thread, a warp, a block and several blocks hold, and odd sizes
 CLASSES = [1, 2, 3, 5, 8, 17, 31, 32, 33, 64, 65, 127, 200, 255, 256, 257, 511, 1000, 1024, 1025, 2047, 2049, 4096, 8191, 16385, 32768, 50021, 65536, 65537, 131072]
+WIDE = [131073, 270001, 600000]      # beyond what a cluster holds, for the wider types first
 
 
 def logits(rng, n, K, dtype, pad=0, shift=0):
@@ -149,6 +150,19 @@ def test_policy_sizes(pkg, K, dtype):
     z, zd = logits(rng, n, K, DTYPES[dtype])
     check_policy(pkg, rng, z, zd, tau=1.0, beta=0.1, hess=K % 2 == 1)
     check_policy(pkg, rng, z, zd, tau=2.0, beta=0.0, hess=K % 2 == 0, ref=False)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("K", WIDE)
+def test_wide_rows(pkg, K, dtype):
+    rng = np.random.default_rng(K + 3)
+    z, zd = logits(rng, 3, K, DTYPES[dtype], pad=K % 5)
+    ids, t = slots(rng, 3, K, 40)
+    check_distill(pkg.distill_grads(zd, ids.cuda(), t.cuda(), tau=1.5, hess=True), z, ids, t, None, 1.5, False, True)
+    lt = log_probs(t, 0.9)
+    check_distill(pkg.distill_grads(zd, ids.cuda(), lt.cuda(), tail=True), z, ids, lt, None, 1.0, True, False)
+    check_policy(pkg, rng, z, zd, 1.0, 0.1, True)
+    check_preference(pkg, z, zd, torch.tensor([5, 0, K], dtype=torch.int32), torch.tensor([0, 1, 3], dtype=torch.int32))
 
 
 def check_policy(pkg, rng, z, zd, tau, beta, hess, ref=True, w=None):
