@@ -60,11 +60,6 @@ __device__ __forceinline__ float load_t(const void *p, int dtype, long long i) {
 // often are made of, would be infinite
 struct Soft { float m, s; };
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; } // nothing but -inf: every term is 2^-inf
-__device__ __forceinline__ float term(float z, float base, float c) { return exp2f((z - base) * c); }
-__device__ __forceinline__ Soft join(Soft a, Soft b, float c) {
-    const float m = fmaxf(a.m, b.m), base = base_of(m);
-    return {m, a.s * term(a.m, base, c) + b.s * term(b.m, base, c)};
-}
 
 struct RowLoss { float loss, d; }; // loss and its derivative by log p of the class taken
 __device__ __forceinline__ RowLoss policy_row(float lp, float old_lp, float adv, const float *ref, long long i, float lo, float hi, float beta) {
@@ -81,119 +76,141 @@ __device__ __forceinline__ RowLoss policy_row(float lp, float old_lp, float adv,
 
 // ---------------------------------------------------------------------------------- rows in registers
 // A row is cut into granules of 16 bytes, as memory is, not as the row begins: element k sits in granule (k + off) / E, off = elements of the
-// first granule that come before the row.  Elements outside of the row read as -inf and are not written.
-template <typename ZT> struct Pack;
-template <> struct Pack<float> {
-    static constexpr int E = 4;
-    static constexpr uint32_t NONE = 0xff800000u;
-    static __device__ __forceinline__ void get(const uint4 &r, float (&x)[4]) {
-        x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
-    }
-    static __device__ __forceinline__ uint4 put(const float (&x)[4]) {
-        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-    }
-    static __device__ __forceinline__ float largest(const uint4 &r) {
-        return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
-    }
-};
-template <> struct Pack<__nv_bfloat16> {
-    static constexpr int E = 8;
-    static constexpr uint32_t NONE = 0xff80ff80u;
-    static __device__ __forceinline__ void two(uint32_t w, float &a, float &b) { a = __uint_as_float(w << 16); b = __uint_as_float(w & 0xffff0000u); }
-    static __device__ __forceinline__ void get(const uint4 &r, float (&x)[8]) {
-        two(r.x, x[0], x[1]); two(r.y, x[2], x[3]); two(r.z, x[4], x[5]); two(r.w, x[6], x[7]);
-    }
-    static __device__ __forceinline__ uint32_t join2(float a, float b) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    }
-    static __device__ __forceinline__ uint4 put(const float (&x)[8]) { return make_uint4(join2(x[0], x[1]), join2(x[2], x[3]), join2(x[4], x[5]), join2(x[6], x[7])); }
-    static __device__ __forceinline__ float largest(const uint4 &r) {
-        const __nv_bfloat162 *v = reinterpret_cast<const __nv_bfloat162 *>(&r);
-        const float2 f = __bfloat1622float2(__hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
-        return fmaxf(f.x, f.y);
-    }
-};
-template <> struct Pack<__half> {
-    static constexpr int E = 8;
-    static constexpr uint32_t NONE = 0xfc00fc00u;
-    static __device__ __forceinline__ void two(uint32_t w, float &a, float &b) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-        a = f.x; b = f.y;
-    }
-    static __device__ __forceinline__ void get(const uint4 &r, float (&x)[8]) {
-        two(r.x, x[0], x[1]); two(r.y, x[2], x[3]); two(r.z, x[4], x[5]); two(r.w, x[6], x[7]);
-    }
-    static __device__ __forceinline__ uint32_t join2(float a, float b) {
-        const __half2 v = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    }
-    static __device__ __forceinline__ uint4 put(const float (&x)[8]) { return make_uint4(join2(x[0], x[1]), join2(x[2], x[3]), join2(x[4], x[5]), join2(x[6], x[7])); }
-    static __device__ __forceinline__ float largest(const uint4 &r) {
-        const __half2 *v = reinterpret_cast<const __half2 *>(&r);
-        const float2 f = __half22float2(__hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
-        return fmaxf(f.x, f.y);
-    }
-};
-
-// Where a row lies
-template <typename ZT> struct RowAt {
-    static constexpr int E = Pack<ZT>::E;
-    const ZT *z;
-    ZT *g, *h;
-    const char *lo, *hi;    // the array's ends
-    int K, off, nvec;
-    bool gv, hv;            // whole granules of g, h can be written: they begin where those of z do
-    __device__ __forceinline__ RowAt(const SoftArgs &a, long long row) {
-        z = static_cast<const ZT *>(a.z) + row * a.ldz;
-        g = a.g ? static_cast<ZT *>(a.g) + row * a.ldg : nullptr;
-        h = a.h ? static_cast<ZT *>(a.h) + row * a.ldh : nullptr;
-        lo = static_cast<const char *>(a.z);
-        hi = reinterpret_cast<const char *>(static_cast<const ZT *>(a.z) + (a.n - 1) * a.ldz + a.K);
-        K = a.K;
-        off = (int)((uintptr_t)z & 15) / (int)sizeof(ZT);
-        nvec = (K + off + E - 1) / E;
-        gv = ((((uintptr_t)g) ^ (uintptr_t)z) & 15) == 0;
-        hv = ((((uintptr_t)h) ^ (uintptr_t)z) & 15) == 0;
-    }
-    __device__ __forceinline__ bool inside(int v) const { return v * E >= off && v * E - off + E <= K; }
-    __device__ __forceinline__ uint4 load(int v) const {
-        const char *p = reinterpret_cast<const char *>(z - off) + (size_t)v * 16;
-        if (inside(v)) return fetch(p);
-        // the ends of a row: a granule that belongs to the array is read whole, else element by element
-        uint4 r = make_uint4(Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE);
-        ZT *x = reinterpret_cast<ZT *>(&r);
-        if (p >= lo && p + 16 <= hi) {
-            const uint4 q = fetch(p);
-            const ZT *y = reinterpret_cast<const ZT *>(&q);
-#pragma unroll
-            for (int e = 0; e < E; ++e) if ((unsigned)(v * E - off + e) < (unsigned)K) x[e] = y[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) if ((unsigned)(v * E - off + e) < (unsigned)K) x[e] = z[v * E - off + e];
-        }
-        return r;
-    }
-    static __device__ __forceinline__ uint4 fetch(const char *p) { return __ldg(reinterpret_cast<const uint4 *>(p)); }
-    __device__ __forceinline__ void store(ZT *o, bool whole, int v, const float (&x)[E]) const {
-        if (whole && inside(v)) { *reinterpret_cast<uint4 *>(o + (v * E - off)) = Pack<ZT>::put(x); return; }
-#pragma unroll
-        for (int e = 0; e < E; ++e) if ((unsigned)(v * E - off + e) < (unsigned)K) o[v * E - off + e] = from_f<ZT>(x[e]);
-    }
-    __device__ __forceinline__ void fill(int v, float value) const {
-        float x[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = value;
-        if (g) store(g, gv, v, x);
-        if (h) store(h, hv, v, x);
-    }
-};
-
+// first granule that come before the row.  The first and the last granule may belong to the row in part: their elements go one by one.
+typedef unsigned long long f2; // two floats side by side: one instruction works on both
+__device__ __forceinline__ f2 pair(float a, float b) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void split(f2 r, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ float ex2(float x) { // of results below 2^-126 nothing is left
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ f2 ex2_2(f2 x) {
+    float a, b;
+    split(x, a, b);
+    return pair(ex2(a), ex2(b));
+}
+template <typename ZT> struct Pack;
+template <> struct Pack<float> {
+    static constexpr int E = 4;
+    static constexpr uint32_t NONE = 0xff800000u;
+    static __device__ __forceinline__ void get(const uint4 &r, f2 (&x)[2]) {
+        x[0] = pair(__uint_as_float(r.x), __uint_as_float(r.y));
+        x[1] = pair(__uint_as_float(r.z), __uint_as_float(r.w));
+    }
+    static __device__ __forceinline__ uint4 put(const f2 (&x)[2]) {
+        float a, b, c, d;
+        split(x[0], a, b); split(x[1], c, d);
+        return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
+    }
+    struct Most { // the largest of many granules
+        float m = -INFINITY;
+        __device__ __forceinline__ void see(const uint4 &r) {
+            m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w))));
+        }
+        __device__ __forceinline__ float get() const { return m; }
+    };
+};
+template <> struct Pack<__nv_bfloat16> {
+    static constexpr int E = 8;
+    static constexpr uint32_t NONE = 0xff80ff80u;
+    static __device__ __forceinline__ f2 two(uint32_t w) { return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+    static __device__ __forceinline__ void get(const uint4 &r, f2 (&x)[4]) { x[0] = two(r.x); x[1] = two(r.y); x[2] = two(r.z); x[3] = two(r.w); }
+    static __device__ __forceinline__ uint32_t one(f2 x) {
+        float a, b;
+        split(x, a, b);
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+    static __device__ __forceinline__ uint4 put(const f2 (&x)[4]) { return make_uint4(one(x[0]), one(x[1]), one(x[2]), one(x[3])); }
+    struct Most {
+        __nv_bfloat162 m = __nv_bfloat162(__ushort_as_bfloat16(0xff80), __ushort_as_bfloat16(0xff80));
+        __device__ __forceinline__ void see(const uint4 &r) {
+            const __nv_bfloat162 *v = reinterpret_cast<const __nv_bfloat162 *>(&r);
+            m = __hmax2(m, __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
+        }
+        __device__ __forceinline__ float get() const { const float2 f = __bfloat1622float2(m); return fmaxf(f.x, f.y); }
+    };
+};
+template <> struct Pack<__half> {
+    static constexpr int E = 8;
+    static constexpr uint32_t NONE = 0xfc00fc00u;
+    static __device__ __forceinline__ f2 two(uint32_t w) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+        return pair(f.x, f.y);
+    }
+    static __device__ __forceinline__ void get(const uint4 &r, f2 (&x)[4]) { x[0] = two(r.x); x[1] = two(r.y); x[2] = two(r.z); x[3] = two(r.w); }
+    static __device__ __forceinline__ uint32_t one(f2 x) {
+        float a, b;
+        split(x, a, b);
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+    static __device__ __forceinline__ uint4 put(const f2 (&x)[4]) { return make_uint4(one(x[0]), one(x[1]), one(x[2]), one(x[3])); }
+    struct Most {
+        __half2 m = __half2(__ushort_as_half(0xfc00), __ushort_as_half(0xfc00));
+        __device__ __forceinline__ void see(const uint4 &r) {
+            const __half2 *v = reinterpret_cast<const __half2 *>(&r);
+            m = __hmax2(m, __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
+        }
+        __device__ __forceinline__ float get() const { const float2 f = __half22float2(m); return fmaxf(f.x, f.y); }
+    };
+};
+
+// Where a row lies, and what of it belongs to one group of threads: granules v0 .. v1 - 1, of which vs .. ve - 1 are whole; `ends` elements
+// of the others.
+template <typename ZT> struct RowAt {
+    static constexpr int E = Pack<ZT>::E, H = E / 2;
+    const ZT *z;
+    ZT *g, *h;
+    int K, off, v0, v1, vs, ve, head, ends;
+    bool whole; // whole granules of g and h can be written: they begin where those of z do
+    __device__ __forceinline__ RowAt(const SoftArgs &a, long long row, int rank, int CS) {
+        z = static_cast<const ZT *>(a.z) + row * a.ldz;
+        g = a.g ? static_cast<ZT *>(a.g) + row * a.ldg : nullptr;
+        h = a.h ? static_cast<ZT *>(a.h) + row * a.ldh : nullptr;
+        K = a.K;
+        off = (int)((uintptr_t)z & 15) / (int)sizeof(ZT);
+        const int nvec = (K + off + E - 1) / E, per = CS > 1 ? (nvec + CS - 1) / CS : nvec;
+        v0 = min(rank * per, nvec);
+        v1 = min(v0 + per, nvec);
+        head = v0 == 0 && off > 0 ? min(K, E - off) : 0;
+        vs = v0 + (head > 0);
+        const bool tail = v1 == nvec && v1 > vs && (K + off) % E != 0;
+        ve = v1 - tail;
+        ends = head + (tail ? K - (ve * E - off) : 0);
+        whole = (((g ? (uintptr_t)g ^ (uintptr_t)z : 0) | (h ? (uintptr_t)h ^ (uintptr_t)z : 0)) & 15) == 0;
+    }
+    __device__ __forceinline__ int end_at(int j) const { return j < head ? j : ve * E - off + j - head; } // element of end j
+    __device__ __forceinline__ const uint4 *granules() const { return reinterpret_cast<const uint4 *>(z - off); }
+    __device__ __forceinline__ uint4 load(int v) const { return __ldg(granules() + v); }
+    __device__ __forceinline__ void store(ZT *o, int v, const f2 (&x)[H]) const {
+        if (whole) { reinterpret_cast<uint4 *>(o - off)[v] = Pack<ZT>::put(x); return; }
+#pragma unroll
+        for (int e = 0; e < H; ++e) {
+            float p, q;
+            split(x[e], p, q);
+            o[v * E - off + 2 * e] = from_f<ZT>(p);
+            o[v * E - off + 2 * e + 1] = from_f<ZT>(q);
+        }
+    }
+    __device__ __forceinline__ void fill(int t, int nt, float value) const {
+        f2 x[H];
+#pragma unroll
+        for (int e = 0; e < H; ++e) x[e] = pair(value, value);
+        for (int v = vs + t; v < ve; v += nt) {
+            if (g) store(g, v, x);
+            if (h) store(h, v, x);
+        }
+        for (int j = t; j < ends; j += nt) {
+            if (g) g[end_at(j)] = from_f<ZT>(value);
+            if (h) h[end_at(j)] = from_f<ZT>(value);
+        }
+    }
+};
+
 // joined by `width` lanes that lie side by side, in a fixed order; every one of them gets it
 __device__ __forceinline__ float lanes_sum(float v, int width) {
     for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
@@ -207,16 +224,32 @@ __device__ __forceinline__ Soft lanes_join(Soft r, float c, int width) {
     const float m = lanes_max(r.m, width);
     return {m, lanes_sum(r.s * ex2((r.m - base_of(m)) * c), width)};
 }
+__device__ __forceinline__ Soft join(Soft a, Soft b, float c) {
+    const float m = fmaxf(a.m, b.m), base = base_of(m);
+    return {m, a.s * ex2((a.m - base) * c) + b.s * ex2((b.m - base) * c)};
+}
+__device__ __forceinline__ bool marked(const uint32_t *bits, int b) { return bits[b >> 5] >> (b & 31) & 1u; }
+template <int E> __device__ __forceinline__ unsigned granule_bits(const uint32_t *bits, int u) { return bits[u * E >> 5] >> (u * E & 31) & ((1u << E) - 1u); }
 
-// Maximum and sum of a thread's V granules; `bits(i)`: elements of granule i to leave out.  32-bit elements become their terms (relative to the
+// A thread's part of a row: granules vs + t, vs + t + nt, ..
+template <typename ZT, int V>
+__device__ __forceinline__ void fetch(uint4 (&r)[V], const RowAt<ZT> &at, int t, int nt, bool live) {
+    const uint4 *p = at.granules() + at.vs + t;
+    const int left = live ? at.ve - at.vs - t : 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        r[i] = i * nt < left ? __ldg(p + i * nt) : make_uint4(Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE);
+}
+// `bits`: null, or marks of the elements to leave out, from the first of granule v0.  32-bit elements become their terms (relative to the
 // thread's maximum), so that no exponential is worked out twice; 16-bit ones stay: their terms would take twice the registers.
-template <typename ZT, int V, typename F>
-__device__ __forceinline__ Soft take(uint4 (&r)[V], float c, bool exclude, F bits) {
-    constexpr int E = Pack<ZT>::E;
-    if (exclude) {
+template <typename ZT, int V>
+__device__ __forceinline__ Soft take(uint4 (&r)[V], const RowAt<ZT> &at, float c, const uint32_t *bits, int t, int nt, bool live) {
+    constexpr int E = Pack<ZT>::E, H = E / 2;
+    if (bits) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const unsigned b = bits(i);
+            const int v = at.vs + t + i * nt;
+            const unsigned b = v < at.ve ? granule_bits<E>(bits, v - at.v0) : 0u;
             if (b) {
                 ZT *x = reinterpret_cast<ZT *>(&r[i]);
 #pragma unroll
@@ -224,23 +257,35 @@ __device__ __forceinline__ Soft take(uint4 (&r)[V], float c, bool exclude, F bit
             }
         }
     }
-    float m = -INFINITY;
+    typename Pack<ZT>::Most most;
 #pragma unroll
-    for (int i = 0; i < V; ++i) m = fmaxf(m, Pack<ZT>::largest(r[i]));
+    for (int i = 0; i < V; ++i) most.see(r[i]);
+    float m = most.get();
+    for (int j = t; live && j < at.ends; j += nt) {
+        const int k = at.end_at(j);
+        if (!bits || !marked(bits, k + at.off - at.v0 * E)) m = fmaxf(m, to_f(at.z[k]));
+    }
     const float base = base_of(m);
-    float s[2] = {0.0f, 0.0f};
+    const f2 c2 = pair(c, c), b2 = pair(-base, -base);
+    f2 s[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        float x[E];
+        f2 x[H];
         Pack<ZT>::get(r[i], x);
 #pragma unroll
-        for (int e = 0; e < E; ++e) { x[e] = ex2((x[e] - base) * c); s[e & 1] += x[e]; }
+        for (int e = 0; e < H; ++e) { x[e] = ex2_2(mul2(add2(x[e], b2), c2)); s[e & 1] = add2(s[e & 1], x[e]); }
         if (E == 4) r[i] = Pack<ZT>::put(x);
         else asm volatile("" : "+r"(r[i].x), "+r"(r[i].y), "+r"(r[i].z), "+r"(r[i].w)); // they stay packed: unpacked they would take twice the registers
     }
-    return {m, s[0] + s[1]};
+    float s0, s1;
+    split(add2(s[0], s[1]), s0, s1);
+    s0 += s1;
+    for (int j = t; live && j < at.ends; j += nt) {
+        const int k = at.end_at(j);
+        if (!bits || !marked(bits, k + at.off - at.v0 * E)) s0 += ex2((to_f(at.z[k]) - base) * c);
+    }
+    return {m, s0};
 }
-
 // Slots of a row in shared memory
 struct Slots {
     int *id;            // class, 0-based, -1: none
@@ -320,25 +365,41 @@ __device__ __forceinline__ RowOut class_row(const SoftArgs &a, Soft r, float za,
     o.hw = w * a.inv_tau * a.inv_tau;
     return o;
 }
-// The gradient (and hessian) of a thread's granule v: `x` holds its elements' terms
-template <typename ZT, int KIND, int E>
-__device__ __forceinline__ void put_terms(const SoftArgs &a, const RowAt<ZT> &at, const RowOut &o, int v, const float (&x)[E], float scale, int code) {
-    float y[E];
-    if (at.g) {
-        const float A = o.A * scale;
+// A thread's part of the gradient (and hessian); `scale`: of its terms, where it holds terms
+template <typename ZT, int KIND, int V>
+__device__ __forceinline__ void give(const SoftArgs &a, const RowAt<ZT> &at, const RowOut &o, const uint4 (&r)[V], int t, int nt, float scale, int code) {
+    constexpr int E = Pack<ZT>::E, H = E / 2;
+    constexpr bool terms = E == 4 && KIND != ROW_COEF;
+    const float A = o.A * scale, B = o.B * scale;
+    const f2 c2 = pair(a.c, a.c), b2 = pair(-o.m, -o.m), A2 = pair(A, A);
+    const int special = KIND == ROW_DISTILL ? -1 : code + at.off;
 #pragma unroll
-        for (int e = 0; e < E; ++e) y[e] = x[e] * A;
-        if (KIND != ROW_DISTILL && v == (code + at.off) / E) {
+    for (int i = 0; i < V; ++i) {
+        const int v = at.vs + t + i * nt;
+        if (v >= at.ve) break;
+        f2 x[H], y[H];
+        Pack<ZT>::get(r[i], x);
 #pragma unroll
-            for (int e = 0; e < E; ++e) if (v * E + e == code + at.off) y[e] = -o.mass * expm1f(o.lp); // 1 - p, also where p is close to 1
+        for (int e = 0; e < H; ++e) {
+            if (!terms) x[e] = ex2_2(mul2(add2(x[e], b2), c2));
+            y[e] = mul2(x[e], A2);
         }
-        at.store(at.g, at.gv, v, y);
-    }
-    if (at.h) {
-        const float B = o.B * scale;
+        if (at.g) {
+            at.store(at.g, v, y);
+            if (KIND != ROW_DISTILL && (unsigned)(special - v * E) < (unsigned)E) at.g[code] = from_f<ZT>(-o.mass * expm1f(o.lp)); // 1 - p, also where p is close to 1
+        }
+        if (at.h) {
+            const f2 B2 = pair(B, B), w2 = pair(o.hw, o.hw), minus = pair(-1.0f, -1.0f), one = pair(1.0f, 1.0f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) { const float p = x[e] * B; y[e] = o.hw * p * (1.0f - p); }
-        at.store(at.h, at.hv, v, y);
+            for (int e = 0; e < H; ++e) { const f2 p = mul2(x[e], B2); y[e] = mul2(mul2(p, w2), add2(one, mul2(p, minus))); }
+            at.store(at.h, v, y);
+        }
+    }
+    for (int j = t; j < at.ends; j += nt) {
+        const int k = at.end_at(j);
+        const float e = ex2((to_f(at.z[k]) - o.m) * a.c), p = e * o.B;
+        if (at.g) at.g[k] = from_f<ZT>(KIND != ROW_DISTILL && k == code ? -o.mass * expm1f(o.lp) : e * o.A);
+        if (at.h) at.h[k] = from_f<ZT>(o.hw * p * (1.0f - p));
     }
 }
 // the named classes, after all others have been written
@@ -356,9 +417,9 @@ __device__ __forceinline__ void put_slot(const SoftArgs &a, const RowAt<ZT> &at,
 }
 
 enum { SLOT_SOME = 1, SLOT_BAD = 2, SLOT_TWICE = 4 };
-// Slot j of a row into shared memory; the classes named in granules v0 .. v1 - 1 are marked in `bits` (bit: element from the first of granule v0)
+// Slot j of a row into shared memory; those classes among granules v0 .. v1 - 1 are marked in `bits` (bit: element from the first of granule v0)
 template <typename ZT>
-__device__ __forceinline__ int put_into(const SoftArgs &a, const RowAt<ZT> &at, const Slots &s, uint32_t *bits, long long row, int j, int v0, int v1) {
+__device__ __forceinline__ int put_into(const SoftArgs &a, const RowAt<ZT> &at, const Slots &s, uint32_t *bits, long long row, int j) {
     const uint32_t id = a.ids[row * a.ldt + j];
     const float t = load_t(a.t, a.t_dtype, row * a.ldt + j);
     const bool use = id != 0u && t != -INFINITY, ok = use && id <= (uint32_t)a.K;
@@ -366,11 +427,10 @@ __device__ __forceinline__ int put_into(const SoftArgs &a, const RowAt<ZT> &at, 
     s.t[j] = t;
     s.z[j] = ok ? to_f(at.z[id - 1]) : 0.0f;
     int flags = (use ? SLOT_SOME : 0) | (use && !ok ? SLOT_BAD : 0);
-    const int b = (int)id - 1 + at.off - v0 * RowAt<ZT>::E;
-    if (ok && b >= 0 && b < (v1 - v0) * RowAt<ZT>::E && (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u)) flags |= SLOT_TWICE;
+    const int b = (int)id - 1 + at.off - at.v0 * RowAt<ZT>::E;
+    if (ok && b >= 0 && b < (at.v1 - at.v0) * RowAt<ZT>::E && (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u)) flags |= SLOT_TWICE;
     return flags;
 }
-template <int E> __device__ __forceinline__ unsigned granule_bits(const uint32_t *bits, int u) { return bits[u * E >> 5] >> (u * E & 31) & ((1u << E) - 1u); }
 
 // Rows of up to V granules for each of G lanes (a power of two up to 32): 32 / G rows a warp, 8 warps a CTA.
 template <typename ZT, int KIND, int V>
@@ -381,7 +441,7 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
     const long long row0 = (long long)blockIdx.x * (256 / G) + group;
     const bool there = row0 < a.n;
     const long long row = there ? row0 : a.n - 1;
-    const RowAt<ZT> at(a, row);
+    const RowAt<ZT> at(a, row, 0, 1);
     unsigned char *mine = s_raw + (size_t)group * (KIND == ROW_DISTILL ? a.T * Slots::BYTES + words * 4 : 0);
     const Slots s(mine, KIND == ROW_DISTILL ? a.T : 0);
     uint32_t *bits = reinterpret_cast<uint32_t *>(mine + (size_t)a.T * Slots::BYTES);
@@ -392,15 +452,11 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
     bool live = there && w != 0.0f && (KIND == ROW_DISTILL || id != 0u);
     int flags = 0;
     uint4 r[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int v = lane + i * G;
-        r[i] = live && v < at.nvec ? at.load(v) : make_uint4(Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE);
-    }
+    fetch<ZT, V>(r, at, lane, G, live);
     if (KIND == ROW_DISTILL) {
         for (int i = lane; i < words; i += G) bits[i] = 0u;
         __syncwarp();
-        if (live) for (int j = lane; j < a.T; j += G) flags |= put_into(a, at, s, bits, row, j, 0, at.nvec);
+        if (live) for (int j = lane; j < a.T; j += G) flags |= put_into(a, at, s, bits, row, j);
         for (int o = G >> 1; o > 0; o >>= 1) flags |= __shfl_xor_sync(FULL, flags, o);
         __syncwarp();
         live = live && (flags & SLOT_SOME);
@@ -410,7 +466,7 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
     const float za = code >= 0 ? to_f(at.z[code]) : 0.0f;
     if (there && !whole) {
         const float value = live ? NAN : 0.0f;
-        if (KIND != ROW_LOGP) for (int v = lane; v < at.nvec; v += G) at.fill(v, value);
+        if (KIND != ROW_LOGP) at.fill(lane, G, value);
         if (lane == 0) {
             if (KIND != ROW_COEF && a.loss) a.loss[row] = value;
             if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = value;
@@ -425,9 +481,7 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
             o.m = base_of(st.x); o.B = st.y; o.lp = a.logp[row]; o.mass = w; o.A = -w * st.y;
         }
     } else {
-        mine_r = take<ZT, V>(r, a.c, KIND == ROW_DISTILL && a.tail && whole, [&](int i) {
-            const int v = lane + i * G;
-            return v < at.nvec ? granule_bits<E>(bits, v) : 0u; });
+        mine_r = take<ZT, V>(r, at, a.c, KIND == ROW_DISTILL && a.tail && whole ? bits : nullptr, lane, G, whole);
         all = lanes_join(mine_r, a.c, G);
         if (KIND == ROW_DISTILL) { if (!whole) for (int j = lane; j < a.T; j += G) s.id[j] = -1; __syncwarp(); o = slots_row(a, s, all, flags & SLOT_TWICE, w, lane, G, true); }
         else if (whole) o = class_row<KIND>(a, all, za, row, w);
@@ -439,21 +493,7 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
             if (KIND == ROW_LOGP) a.stat[row] = make_float2(all.m, o.B);
         }
         const float scale = E == 4 && KIND != ROW_COEF ? ex2((mine_r.m - o.m) * a.c) : 1.0f;
-        if (KIND != ROW_LOGP && (at.g || at.h)) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int v = lane + i * G;
-                if (v < at.nvec) {
-                    float x[E];
-                    Pack<ZT>::get(r[i], x);
-                    if (E == 8 || KIND == ROW_COEF) {
-#pragma unroll
-                        for (int e = 0; e < E; ++e) x[e] = ex2((x[e] - o.m) * a.c);
-                    }
-                    put_terms<ZT, KIND>(a, at, o, v, x, scale, code);
-                }
-            }
-        }
+        if (KIND != ROW_LOGP) give<ZT, KIND, V>(a, at, o, r, lane, G, scale, code);
     }
     if (KIND == ROW_DISTILL) {
         __syncwarp();
@@ -481,7 +521,7 @@ __device__ __forceinline__ int cluster_read(const int *p, int rank) {
 
 // One row for a CTA, or for a cluster of CS CTAs, up to V granules a thread.
 template <typename ZT, int KIND, int V>
-__global__ void __launch_bounds__(V > 4 ? 512 : 1024) k_row_ctas(SoftArgs a, int CS, int words) {
+__global__ void __launch_bounds__(V > 4 ? 512 : 1024, V > 4 ? 2 : 1) k_row_ctas(SoftArgs a, int CS, int words) {
     extern __shared__ __align__(16) unsigned char s_raw[];
     __shared__ float2 s_part[32];
     __shared__ float2 s_cta;
@@ -490,8 +530,7 @@ __global__ void __launch_bounds__(V > 4 ? 512 : 1024) k_row_ctas(SoftArgs a, int
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warps = nt >> 5;
     const long long row = blockIdx.x / (unsigned)CS;
     const int rank = CS > 1 ? (int)(blockIdx.x % (unsigned)CS) : 0;
-    const RowAt<ZT> at(a, row);
-    const int per = (at.nvec + CS - 1) / CS, v0 = min(rank * per, at.nvec), v1 = min(v0 + per, at.nvec);
+    const RowAt<ZT> at(a, row, rank, CS);
     const Slots s(s_raw, KIND == ROW_DISTILL ? a.T : 0);
     uint32_t *bits = reinterpret_cast<uint32_t *>(s_raw + (size_t)a.T * Slots::BYTES);
     float w = a.w ? a.w[row * a.w_stride] : 1.0f;
@@ -500,17 +539,13 @@ __global__ void __launch_bounds__(V > 4 ? 512 : 1024) k_row_ctas(SoftArgs a, int
     if (KIND != ROW_DISTILL) id = a.code[row * a.p_stride];
     bool live = w != 0.0f && (KIND == ROW_DISTILL || id != 0u);
     uint4 r[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int v = v0 + tid + i * nt;
-        r[i] = live && v < v1 ? at.load(v) : make_uint4(Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE);
-    }
+    fetch<ZT, V>(r, at, tid, nt, live);
     int flags = live && KIND != ROW_DISTILL && id > (uint32_t)a.K ? SLOT_BAD : 0;
     if (KIND == ROW_DISTILL && live) {
         if (tid == 0) s_flags = 0;
         for (int i = tid; i < words; i += nt) bits[i] = 0u;
         __syncthreads();
-        for (int j = tid; j < a.T; j += nt) flags |= put_into(a, at, s, bits, row, j, v0, v1);
+        for (int j = tid; j < a.T; j += nt) flags |= put_into(a, at, s, bits, row, j);
         flags = __reduce_or_sync(FULL, flags);
         if (lane == 0 && flags) atomicOr(&s_flags, flags);
         __syncthreads();
@@ -519,7 +554,7 @@ __global__ void __launch_bounds__(V > 4 ? 512 : 1024) k_row_ctas(SoftArgs a, int
     }
     if (!live || (flags & SLOT_BAD)) {
         const float value = live ? NAN : 0.0f;
-        if (KIND != ROW_LOGP) for (int v = v0 + tid; v < v1; v += nt) at.fill(v, value);
+        if (KIND != ROW_LOGP) at.fill(tid, nt, value);
         if (tid == 0 && rank == 0) {
             if (KIND != ROW_COEF && a.loss) a.loss[row] = value;
             if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = value;
@@ -535,9 +570,7 @@ __global__ void __launch_bounds__(V > 4 ? 512 : 1024) k_row_ctas(SoftArgs a, int
         const float2 st = a.stat[row];
         o.m = base_of(st.x); o.B = st.y; o.lp = a.logp[row]; o.mass = w; o.A = -w * st.y;
     } else {
-        mine = take<ZT, V>(r, a.c, KIND == ROW_DISTILL && a.tail, [&](int i) {
-            const int v = v0 + tid + i * nt;
-            return v < v1 ? granule_bits<E>(bits, v - v0) : 0u; });
+        mine = take<ZT, V>(r, at, a.c, KIND == ROW_DISTILL && a.tail ? bits : nullptr, tid, nt, true);
         all = lanes_join(mine, a.c, 32);
         if (lane == 0) s_part[tid >> 5] = make_float2(all.m, all.s);
         __syncthreads();
@@ -562,24 +595,12 @@ __global__ void __launch_bounds__(V > 4 ? 512 : 1024) k_row_ctas(SoftArgs a, int
     }
     if (KIND != ROW_LOGP && (at.g || at.h)) {
         const float scale = E == 4 && KIND != ROW_COEF ? ex2((mine.m - o.m) * a.c) : 1.0f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int v = v0 + tid + i * nt;
-            if (v < v1) {
-                float x[E];
-                Pack<ZT>::get(r[i], x);
-                if (E == 8 || KIND == ROW_COEF) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) x[e] = ex2((x[e] - o.m) * a.c);
-                }
-                put_terms<ZT, KIND>(a, at, o, v, x, scale, code);
-            }
-        }
+        give<ZT, KIND, V>(a, at, o, r, tid, nt, scale, code);
         if (KIND == ROW_DISTILL) {
             __syncthreads();
             for (int j = tid; j < a.T; j += nt) {
                 const int k = s.id[j], v = (k + at.off) / E;
-                if (k >= 0 && v >= v0 && v < v1) put_slot(a, at, o, s, j, flags & SLOT_TWICE, w);
+                if (k >= 0 && v >= at.v0 && v < at.v1) put_slot(a, at, o, s, j, flags & SLOT_TWICE, w);
             }
         }
     }
@@ -595,7 +616,7 @@ __global__ void __launch_bounds__(512) k_row_walk(SoftArgs a, int words) {
     constexpr int E = Pack<ZT>::E;
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warps = nt >> 5;
     const long long row = blockIdx.x;
-    const RowAt<ZT> at(a, row);
+    const RowAt<ZT> at(a, row, 0, 1);
     const Slots s(s_raw, KIND == ROW_DISTILL ? a.T : 0);
     uint32_t *bits = reinterpret_cast<uint32_t *>(s_raw + (size_t)a.T * Slots::BYTES);
     float w = a.w ? a.w[row * a.w_stride] : 1.0f;
@@ -608,7 +629,7 @@ __global__ void __launch_bounds__(512) k_row_walk(SoftArgs a, int words) {
         if (tid == 0) s_flags = 0;
         for (int i = tid; i < words; i += nt) bits[i] = 0u;
         __syncthreads();
-        for (int j = tid; j < a.T; j += nt) flags |= put_into(a, at, s, bits, row, j, 0, at.nvec);
+        for (int j = tid; j < a.T; j += nt) flags |= put_into(a, at, s, bits, row, j);
         flags = __reduce_or_sync(FULL, flags);
         if (lane == 0 && flags) atomicOr(&s_flags, flags);
         __syncthreads();
@@ -617,7 +638,7 @@ __global__ void __launch_bounds__(512) k_row_walk(SoftArgs a, int words) {
     }
     if (!live || (flags & SLOT_BAD)) {
         const float value = live ? NAN : 0.0f;
-        if (KIND != ROW_LOGP) for (int v = tid; v < at.nvec; v += nt) at.fill(v, value);
+        if (KIND != ROW_LOGP) at.fill(tid, nt, value);
         if (tid == 0) {
             if (KIND != ROW_COEF && a.loss) a.loss[row] = value;
             if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = value;
@@ -633,9 +654,13 @@ __global__ void __launch_bounds__(512) k_row_walk(SoftArgs a, int words) {
         o.m = base_of(st.x); o.B = st.y; o.lp = a.logp[row]; o.mass = w; o.A = -w * st.y;
     } else {
         Soft all = {-INFINITY, 0.0f};
-        for (int v = tid; v < at.nvec; v += nt) {
-            uint4 r[1] = {at.load(v)};
-            all = join(all, take<ZT, 1>(r, a.c, KIND == ROW_DISTILL && a.tail, [&](int) { return granule_bits<E>(bits, v); }), a.c);
+        RowAt<ZT> piece = at; // 4 granules a thread at a time, the ends with the last
+        for (piece.vs = at.vs; piece.vs < at.ve || piece.vs == at.vs; piece.vs += 4 * nt) {
+            const bool last = piece.vs + 4 * nt >= at.ve;
+            piece.ends = last ? at.ends : 0;
+            uint4 r[4];
+            fetch<ZT, 4>(r, piece, tid, nt, true);
+            all = join(all, take<ZT, 4>(r, piece, a.c, KIND == ROW_DISTILL && a.tail ? bits : nullptr, tid, nt, true), a.c);
         }
         all = lanes_join(all, a.c, 32);
         if (lane == 0) s_part[tid >> 5] = make_float2(all.m, all.s);
@@ -651,13 +676,14 @@ __global__ void __launch_bounds__(512) k_row_walk(SoftArgs a, int words) {
         if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = o.lp;
     }
     if (KIND == ROW_LOGP || !(at.g || at.h)) return;
-    for (int v = tid; v < at.nvec; v += nt) {
-        float x[E];
-        const uint4 r = at.load(v);
-        Pack<ZT>::get(r, x);
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = ex2((x[e] - o.m) * a.c);
-        put_terms<ZT, KIND>(a, at, o, v, x, 1.0f, code);
+    RowAt<ZT> piece = at;
+    for (piece.vs = at.vs; piece.vs < at.ve || piece.vs == at.vs; piece.vs += 4 * nt) {
+        piece.ends = piece.vs + 4 * nt >= at.ve ? at.ends : 0;
+        uint4 r[4];
+        fetch<ZT, 4>(r, piece, tid, nt, true);
+        float scale = 1.0f;
+        if (E == 4 && KIND != ROW_COEF) scale = ex2((take<ZT, 4>(r, piece, a.c, nullptr, tid, nt, false).m - o.m) * a.c);
+        give<ZT, KIND, 4>(a, piece, o, r, tid, nt, scale, code);
     }
     if (KIND == ROW_DISTILL) {
         __syncthreads();
