@@ -8,6 +8,7 @@
 #include <cuda_fp16.h>
 #include <algorithm>
 #include <math.h>
+#include <mutex>
 
 namespace {
 
@@ -56,18 +57,21 @@ __device__ __forceinline__ float load_t(const void *p, int dtype, long long i) {
     return static_cast<const float *>(p)[i];
 }
 
-// Maximum and sum of 2^(c (z - max)) of what has been seen.  The difference comes first: products c z of the type's lowest value, which masks
-// often are made of, would be infinite
+// Maximum m and sum of 2^(c z - M), M = round(c m), of what has been seen: a multiply-add and an exponential per term.
 struct Soft { float m, s; };
-__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; } // nothing but -inf: every term is 2^-inf
+__device__ __forceinline__ float base_of(float m, float c) { const float M = __fmul_rn(m, c); return M == -INFINITY ? 0.0f : M; } // nothing seen: every term is 2^-inf
+__device__ __forceinline__ float rise(float m, float c, float base) { return __fmul_rn(m, c) - base; } // between two M: the product rounded, never a multiply-add
+// Where M's rounding would reach the exponents, or the products overflow (masks are often made of the type's lowest value), a part of a row
+// sees nothing: its terms are 2^-inf.  When that is the largest prediction of the whole row, it is looked at again, less its maximum.
+__device__ __forceinline__ bool is_far(float m, float c) { return fabsf(m) * c > 1.0e9f && m != -INFINITY; }
 
 struct RowLoss { float loss, d; }; // loss and its derivative by log p of the class taken
-__device__ __forceinline__ RowLoss policy_row(float lp, float old_lp, float adv, const float *ref, long long i, float lo, float hi, float beta) {
+__device__ __forceinline__ RowLoss policy_row(float lp, float old_lp, float adv, bool has_ref, float ref, float lo, float hi, float beta) {
     const float r = expf(lp - old_lp), u = r * adv, cl = fminf(fmaxf(r, 1.0f - lo), 1.0f + hi) * adv;
     RowLoss o = {u <= cl ? -u : -cl, u <= cl ? -u : 0.0f};
     if (u != u) o = {u, u};
-    if (ref) {
-        const float x = ref[i] - lp, e = expm1f(x);
+    if (has_ref) {
+        const float x = ref - lp, e = expm1f(x);
         o.loss += beta * (e - x);
         o.d -= beta * e;
     }
@@ -77,33 +81,47 @@ __device__ __forceinline__ RowLoss policy_row(float lp, float old_lp, float adv,
 // ---------------------------------------------------------------------------------- rows in registers
 // A row is cut into granules of 16 bytes, as memory is, not as the row begins: element k sits in granule (k + off) / E, off = elements of the
 // first granule that come before the row.  The first and the last granule may belong to the row in part: their elements go one by one.
-typedef unsigned long long f2; // two floats side by side: one instruction works on both
-__device__ __forceinline__ f2 pair(float a, float b) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
-__device__ __forceinline__ void split(f2 r, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ float ex2(float x) { // of results below 2^-126 nothing is left
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+typedef unsigned long long f2; // two floats side by side: one instruction works on both
+__device__ __forceinline__ f2 pair(float a, float b) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void split(f2 r, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ f2 ex2_2(f2 x) {
     float a, b;
     split(x, a, b);
     return pair(ex2(a), ex2(b));
 }
+struct Two {
+    template <typename P, int E> static __device__ __forceinline__ void get(const uint4 &r, f2 (&x)[E / 2]) {
+        float y[E];
+        P::get(r, y);
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) x[e] = pair(y[2 * e], y[2 * e + 1]);
+    }
+    template <typename P, int E> static __device__ __forceinline__ uint4 put(const f2 (&x)[E / 2]) {
+        float y[E];
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) split(x[e], y[2 * e], y[2 * e + 1]);
+        return P::put(y);
+    }
+};
 template <typename ZT> struct Pack;
 template <> struct Pack<float> {
     static constexpr int E = 4;
+    static __device__ __forceinline__ void get2(const uint4 &r, f2 (&x)[2]) { Two::get<Pack, 4>(r, x); }
+    static __device__ __forceinline__ uint4 put2(const f2 (&x)[2]) { return Two::put<Pack, 4>(x); }
     static constexpr uint32_t NONE = 0xff800000u;
-    static __device__ __forceinline__ void get(const uint4 &r, f2 (&x)[2]) {
-        x[0] = pair(__uint_as_float(r.x), __uint_as_float(r.y));
-        x[1] = pair(__uint_as_float(r.z), __uint_as_float(r.w));
+    static __device__ __forceinline__ void get(const uint4 &r, float (&x)[4]) {
+        x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
     }
-    static __device__ __forceinline__ uint4 put(const f2 (&x)[2]) {
-        float a, b, c, d;
-        split(x[0], a, b); split(x[1], c, d);
-        return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
+    static __device__ __forceinline__ uint4 put(const float (&x)[4]) {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
     }
     struct Most { // the largest of many granules
         float m = -INFINITY;
@@ -115,16 +133,18 @@ template <> struct Pack<float> {
 };
 template <> struct Pack<__nv_bfloat16> {
     static constexpr int E = 8;
+    static __device__ __forceinline__ void get2(const uint4 &r, f2 (&x)[4]) { Two::get<Pack, 8>(r, x); }
+    static __device__ __forceinline__ uint4 put2(const f2 (&x)[4]) { return Two::put<Pack, 8>(x); }
     static constexpr uint32_t NONE = 0xff80ff80u;
-    static __device__ __forceinline__ f2 two(uint32_t w) { return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
-    static __device__ __forceinline__ void get(const uint4 &r, f2 (&x)[4]) { x[0] = two(r.x); x[1] = two(r.y); x[2] = two(r.z); x[3] = two(r.w); }
-    static __device__ __forceinline__ uint32_t one(f2 x) {
-        float a, b;
-        split(x, a, b);
+    static __device__ __forceinline__ void two(uint32_t w, float &a, float &b) { a = __uint_as_float(w << 16); b = __uint_as_float(w & 0xffff0000u); }
+    static __device__ __forceinline__ void get(const uint4 &r, float (&x)[8]) {
+        two(r.x, x[0], x[1]); two(r.y, x[2], x[3]); two(r.z, x[4], x[5]); two(r.w, x[6], x[7]);
+    }
+    static __device__ __forceinline__ uint32_t one(float a, float b) {
         const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t *>(&v);
     }
-    static __device__ __forceinline__ uint4 put(const f2 (&x)[4]) { return make_uint4(one(x[0]), one(x[1]), one(x[2]), one(x[3])); }
+    static __device__ __forceinline__ uint4 put(const float (&x)[8]) { return make_uint4(one(x[0], x[1]), one(x[2], x[3]), one(x[4], x[5]), one(x[6], x[7])); }
     struct Most {
         __nv_bfloat162 m = __nv_bfloat162(__ushort_as_bfloat16(0xff80), __ushort_as_bfloat16(0xff80));
         __device__ __forceinline__ void see(const uint4 &r) {
@@ -136,19 +156,21 @@ template <> struct Pack<__nv_bfloat16> {
 };
 template <> struct Pack<__half> {
     static constexpr int E = 8;
+    static __device__ __forceinline__ void get2(const uint4 &r, f2 (&x)[4]) { Two::get<Pack, 8>(r, x); }
+    static __device__ __forceinline__ uint4 put2(const f2 (&x)[4]) { return Two::put<Pack, 8>(x); }
     static constexpr uint32_t NONE = 0xfc00fc00u;
-    static __device__ __forceinline__ f2 two(uint32_t w) {
+    static __device__ __forceinline__ void two(uint32_t w, float &a, float &b) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-        return pair(f.x, f.y);
+        a = f.x; b = f.y;
     }
-    static __device__ __forceinline__ void get(const uint4 &r, f2 (&x)[4]) { x[0] = two(r.x); x[1] = two(r.y); x[2] = two(r.z); x[3] = two(r.w); }
-    static __device__ __forceinline__ uint32_t one(f2 x) {
-        float a, b;
-        split(x, a, b);
+    static __device__ __forceinline__ void get(const uint4 &r, float (&x)[8]) {
+        two(r.x, x[0], x[1]); two(r.y, x[2], x[3]); two(r.z, x[4], x[5]); two(r.w, x[6], x[7]);
+    }
+    static __device__ __forceinline__ uint32_t one(float a, float b) {
         const __half2 v = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t *>(&v);
     }
-    static __device__ __forceinline__ uint4 put(const f2 (&x)[4]) { return make_uint4(one(x[0]), one(x[1]), one(x[2]), one(x[3])); }
+    static __device__ __forceinline__ uint4 put(const float (&x)[8]) { return make_uint4(one(x[0], x[1]), one(x[2], x[3]), one(x[4], x[5]), one(x[6], x[7])); }
     struct Most {
         __half2 m = __half2(__ushort_as_half(0xfc00), __ushort_as_half(0xfc00));
         __device__ __forceinline__ void see(const uint4 &r) {
@@ -162,7 +184,7 @@ template <> struct Pack<__half> {
 // Where a row lies, and what of it belongs to one group of threads: granules v0 .. v1 - 1, of which vs .. ve - 1 are whole; `ends` elements
 // of the others.
 template <typename ZT> struct RowAt {
-    static constexpr int E = Pack<ZT>::E, H = E / 2;
+    static constexpr int E = Pack<ZT>::E;
     const ZT *z;
     ZT *g, *h;
     int K, off, v0, v1, vs, ve, head, ends;
@@ -186,20 +208,15 @@ template <typename ZT> struct RowAt {
     __device__ __forceinline__ int end_at(int j) const { return j < head ? j : ve * E - off + j - head; } // element of end j
     __device__ __forceinline__ const uint4 *granules() const { return reinterpret_cast<const uint4 *>(z - off); }
     __device__ __forceinline__ uint4 load(int v) const { return __ldg(granules() + v); }
-    __device__ __forceinline__ void store(ZT *o, int v, const f2 (&x)[H]) const {
+    __device__ __forceinline__ void store(ZT *o, int v, const float (&x)[E]) const {
         if (whole) { reinterpret_cast<uint4 *>(o - off)[v] = Pack<ZT>::put(x); return; }
 #pragma unroll
-        for (int e = 0; e < H; ++e) {
-            float p, q;
-            split(x[e], p, q);
-            o[v * E - off + 2 * e] = from_f<ZT>(p);
-            o[v * E - off + 2 * e + 1] = from_f<ZT>(q);
-        }
+        for (int e = 0; e < E; ++e) o[v * E - off + e] = from_f<ZT>(x[e]);
     }
     __device__ __forceinline__ void fill(int t, int nt, float value) const {
-        f2 x[H];
+        float x[E];
 #pragma unroll
-        for (int e = 0; e < H; ++e) x[e] = pair(value, value);
+        for (int e = 0; e < E; ++e) x[e] = value;
         for (int v = vs + t; v < ve; v += nt) {
             if (g) store(g, v, x);
             if (h) store(h, v, x);
@@ -217,16 +234,21 @@ __device__ __forceinline__ float lanes_sum(float v, int width) {
     return v;
 }
 __device__ __forceinline__ float lanes_max(float v, int width) {
+    if (width == 32) {
+        float m;
+        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+        return m;
+    }
     for (int o = width >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
     return v;
 }
 __device__ __forceinline__ Soft lanes_join(Soft r, float c, int width) {
     const float m = lanes_max(r.m, width);
-    return {m, lanes_sum(r.s * ex2((r.m - base_of(m)) * c), width)};
+    return {m, lanes_sum(r.s * ex2(rise(r.m, c, base_of(m, c))), width)};
 }
 __device__ __forceinline__ Soft join(Soft a, Soft b, float c) {
-    const float m = fmaxf(a.m, b.m), base = base_of(m);
-    return {m, a.s * ex2((a.m - base) * c) + b.s * ex2((b.m - base) * c)};
+    const float m = fmaxf(a.m, b.m), base = base_of(m, c);
+    return {m, a.s * ex2(rise(a.m, c, base)) + b.s * ex2(rise(b.m, c, base))};
 }
 __device__ __forceinline__ bool marked(const uint32_t *bits, int b) { return bits[b >> 5] >> (b & 31) & 1u; }
 template <int E> __device__ __forceinline__ unsigned granule_bits(const uint32_t *bits, int u) { return bits[u * E >> 5] >> (u * E & 31) & ((1u << E) - 1u); }
@@ -235,28 +257,48 @@ template <int E> __device__ __forceinline__ unsigned granule_bits(const uint32_t
 template <typename ZT, int V>
 __device__ __forceinline__ void fetch(uint4 (&r)[V], const RowAt<ZT> &at, int t, int nt, bool live) {
     const uint4 *p = at.granules() + at.vs + t;
-    const int left = live ? at.ve - at.vs - t : 0;
+    const int left = live ? at.ve - at.vs : 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-        r[i] = i * nt < left ? __ldg(p + i * nt) : make_uint4(Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE);
+    for (int i = 0; i < V; ++i) {
+        if ((i + 1) * nt <= left) r[i] = __ldg(p + i * nt);        // the same for all threads of the row
+        else r[i] = i * nt + t < left ? __ldg(p + i * nt) : make_uint4(Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE);
+    }
+}
+template <typename ZT, int V>
+__device__ __forceinline__ void leave_out(uint4 (&r)[V], const RowAt<ZT> &at, const uint32_t *bits, int t, int nt) {
+    constexpr int E = Pack<ZT>::E;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int v = at.vs + t + i * nt;
+        const unsigned b = v < at.ve ? granule_bits<E>(bits, v - at.v0) : 0u;
+        if (b) {
+            ZT *x = reinterpret_cast<ZT *>(&r[i]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) if (b >> e & 1u) x[e] = from_f<ZT>(-INFINITY);
+        }
+    }
+}
+template <typename ZT, int V>
+__device__ __forceinline__ float terms_of(uint4 (&r)[V], float c, float nb) {
+    constexpr int E = Pack<ZT>::E;
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        float x[E];
+        Pack<ZT>::get(r[i], x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) { x[e] = ex2(fmaf(x[e], c, nb)); s[e & 1] += x[e]; }
+        if (E == 4) r[i] = Pack<ZT>::put(x);
+        else asm volatile("" : "+r"(r[i].x), "+r"(r[i].y), "+r"(r[i].z), "+r"(r[i].w)); // they stay packed: unpacked they would take twice the registers
+    }
+    return s[0] + s[1];
 }
 // `bits`: null, or marks of the elements to leave out, from the first of granule v0.  32-bit elements become their terms (relative to the
 // thread's maximum), so that no exponential is worked out twice; 16-bit ones stay: their terms would take twice the registers.
 template <typename ZT, int V>
 __device__ __forceinline__ Soft take(uint4 (&r)[V], const RowAt<ZT> &at, float c, const uint32_t *bits, int t, int nt, bool live) {
-    constexpr int E = Pack<ZT>::E, H = E / 2;
-    if (bits) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int v = at.vs + t + i * nt;
-            const unsigned b = v < at.ve ? granule_bits<E>(bits, v - at.v0) : 0u;
-            if (b) {
-                ZT *x = reinterpret_cast<ZT *>(&r[i]);
-#pragma unroll
-                for (int e = 0; e < E; ++e) if (b >> e & 1u) x[e] = from_f<ZT>(-INFINITY);
-            }
-        }
-    }
+    constexpr int E = Pack<ZT>::E;
+    if (bits) leave_out<ZT, V>(r, at, bits, t, nt);
     typename Pack<ZT>::Most most;
 #pragma unroll
     for (int i = 0; i < V; ++i) most.see(r[i]);
@@ -265,27 +307,72 @@ __device__ __forceinline__ Soft take(uint4 (&r)[V], const RowAt<ZT> &at, float c
         const int k = at.end_at(j);
         if (!bits || !marked(bits, k + at.off - at.v0 * E)) m = fmaxf(m, to_f(at.z[k]));
     }
-    const float base = base_of(m);
-    const f2 c2 = pair(c, c), b2 = pair(-base, -base);
-    f2 s[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        f2 x[H];
-        Pack<ZT>::get(r[i], x);
-#pragma unroll
-        for (int e = 0; e < H; ++e) { x[e] = ex2_2(mul2(add2(x[e], b2), c2)); s[e & 1] = add2(s[e & 1], x[e]); }
-        if (E == 4) r[i] = Pack<ZT>::put(x);
-        else asm volatile("" : "+r"(r[i].x), "+r"(r[i].y), "+r"(r[i].z), "+r"(r[i].w)); // they stay packed: unpacked they would take twice the registers
-    }
-    float s0, s1;
-    split(add2(s[0], s[1]), s0, s1);
-    s0 += s1;
+    const float nb = is_far(m, c) ? -INFINITY : -base_of(m, c);
+    float sum = terms_of<ZT, V>(r, c, nb);
     for (int j = t; live && j < at.ends; j += nt) {
         const int k = at.end_at(j);
-        if (!bits || !marked(bits, k + at.off - at.v0 * E)) s0 += ex2((to_f(at.z[k]) - base) * c);
+        if (!bits || !marked(bits, k + at.off - at.v0 * E)) sum += ex2(fmaf(to_f(at.z[k]), c, nb));
     }
-    return {m, s0};
+    return {m, sum};
 }
+// The part again, less the row's maximum.  Differences of 16-bit numbers are rounded to their type: where |c m| is above 1e9 two of them are
+// equal or 2^11 and more exponents apart, before as after.
+template <typename ZT, int V>
+__device__ __noinline__ void less_mem(uint4 (&r)[V], const RowAt<ZT> &at, float m, const uint32_t *bits, int t, int nt) {
+    constexpr int E = Pack<ZT>::E;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int v = at.vs + t + i * nt;
+        if (v >= at.ve) continue;
+        r[i] = at.load(v);
+        const unsigned b = bits ? granule_bits<E>(bits, v - at.v0) : 0u;
+        ZT *x = reinterpret_cast<ZT *>(&r[i]);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = from_f<ZT>(b >> e & 1u ? -INFINITY : to_f(x[e]) - m);
+    }
+}
+template <typename ZT, int V>
+__device__ __noinline__ float take_far_mem(uint4 (&r)[V], const RowAt<ZT> &at, float m, float c, const uint32_t *bits, int t, int nt) {
+    constexpr int E = Pack<ZT>::E;
+    less_mem<ZT, V>(r, at, m, bits, t, nt);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        float x[E];
+        Pack<ZT>::get(r[i], x);
+        const bool in = at.vs + t + i * nt < at.ve;
+#pragma unroll
+        for (int e = 0; e < E; ++e) { x[e] = in ? ex2(x[e] * c) : 0.0f; sum += x[e]; }
+        if (E == 4) r[i] = Pack<ZT>::put(x);
+    }
+    for (int j = t; j < at.ends; j += nt) {
+        const int k = at.end_at(j);
+        if (!bits || !marked(bits, k + at.off - at.v0 * E)) sum += ex2((to_f(at.z[k]) - m) * c);
+    }
+    return sum;
+}
+
+// calls: what they are given lies in memory, and only there does it
+template <typename ZT, int V>
+__device__ __forceinline__ void less(uint4 (&r)[V], const RowAt<ZT> &at, float m, const uint32_t *bits, int t, int nt) {
+    uint4 q[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) q[i] = r[i];
+    less_mem<ZT, V>(q, at, m, bits, t, nt);
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = q[i];
+}
+template <typename ZT, int V>
+__device__ __forceinline__ float take_far(uint4 (&r)[V], const RowAt<ZT> &at, float m, float c, const uint32_t *bits, int t, int nt) {
+    uint4 q[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) q[i] = make_uint4(0u, 0u, 0u, 0u);
+    const float sum = take_far_mem<ZT, V>(q, at, m, c, bits, t, nt);
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = q[i];
+    return sum;
+}
+
 // Slots of a row in shared memory
 struct Slots {
     int *id;            // class, 0-based, -1: none
@@ -298,8 +385,11 @@ struct Slots {
         z = t + T; q = z + T; lp = q + T;
     }
 };
+constexpr float LN2 = 0.693147180559945309f;
 struct RowOut {
-    float m, A, B;      // gradient A e and probability B e of the classes that are not named, e = 2^(c (z - m))
+    float M, A, B;      // gradient A e and probability B e of the classes that are not named, e = 2^(c (z - shift) - M)
+    float shift;        // 0, or the maximum of a row that is far away
+    float special;      // gradient of the class taken
     float mass;         // distillation: sum of the teacher's probabilities; else: factor of (delta - p)
     float hw;           // hessian hw p (1 - p)
     float lp;           // log p of the class taken
@@ -310,97 +400,126 @@ __device__ __forceinline__ bool first_slot(const Slots &s, int j) {
     return true;
 }
 // r: what the scan found.  `width` lanes share the slots; `keep`: these lanes write q and lp
-__device__ __forceinline__ RowOut slots_row(const SoftArgs &a, const Slots &s, Soft r, bool dup, float w, int lane, int width, bool keep) {
+__device__ __forceinline__ RowOut slots_row(const SoftArgs &a, const Slots &s, Soft r, float shift, bool dup, float w, int lane, int width, bool keep) {
     const float c = a.c;
     float tmax = -INFINITY, zmax = r.m;
-    for (int j = lane; j < a.T; j += width) if (s.id[j] >= 0) { tmax = fmaxf(tmax, s.t[j]); zmax = fmaxf(zmax, s.z[j]); }
+    for (int j = lane; j < a.T; j += width) if (s.id[j] >= 0) { tmax = fmaxf(tmax, s.t[j]); zmax = fmaxf(zmax, s.z[j] - shift); }
     if (!a.tail) tmax = lanes_max(tmax, width);
     zmax = lanes_max(zmax, width);
-    const float base = base_of(zmax);
+    const float base = base_of(zmax, c);
     float Q = 0.0f, named = 0.0f;
     for (int j = lane; j < a.T; j += width) {
         if (s.id[j] < 0) continue;
         Q += a.tail ? expf(s.t[j]) : expf((s.t[j] - tmax) * a.inv_tau);
-        if (a.tail && (!dup || first_slot(s, j))) named += ex2((s.z[j] - base) * c);
+        if (a.tail && (!dup || first_slot(s, j))) named += ex2(fmaf(s.z[j] - shift, c, -base));
     }
     Q = lanes_sum(Q, width);
     Soft all = r;
-    if (a.tail) all = {zmax, lanes_sum(named, width) + r.s * ex2((r.m - base) * c)};
-    const float ls = logf(all.s), lq = logf(Q);
+    if (a.tail) all = {zmax, lanes_sum(named, width) + r.s * ex2(rise(r.m, c, base))};
+    const float M = base_of(all.m, c), ls = log2f(all.s), lq = logf(Q);
     float loss = 0.0f;
     for (int j = lane; j < a.T; j += width) {
         if (s.id[j] < 0) continue;
-        const float lt = a.tail ? s.t[j] : (s.t[j] - tmax) * a.inv_tau - lq, q = expf(lt), lp = (s.z[j] - all.m) * a.inv_tau - ls;
+        const float lt = a.tail ? s.t[j] : (s.t[j] - tmax) * a.inv_tau - lq, q = expf(lt), lp = LN2 * (fmaf(s.z[j] - shift, c, -M) - ls);
         if (keep) { s.q[j] = q; s.lp[j] = lp; }
         if (q != 0.0f) loss += q * (lt - lp);
     }
     loss = lanes_sum(loss, width);
     // the rest, when there is any: no class is left where every one is named or ruled out
     const float qt = a.tail && r.m != -INFINITY ? fmaxf(0.0f, 1.0f - Q) : 0.0f;
-    if (qt > 0.0f) loss += qt * (logf(qt) - ((r.m - all.m) * a.inv_tau + logf(r.s) - ls));
+    if (qt > 0.0f) loss += qt * (logf(qt) - LN2 * (rise(r.m, c, M) + log2f(r.s) - ls));
     RowOut o;
-    o.m = base_of(r.m);
+    o.M = base_of(r.m, c);
+    o.shift = shift;
     o.mass = a.tail ? Q + qt : 1.0f;
-    o.B = r.m == -INFINITY ? 0.0f * ls : ex2((r.m - base_of(all.m)) * c) / all.s;
+    o.B = r.m == -INFINITY ? 0.0f * ls : ex2(rise(r.m, c, M)) / all.s;
     o.A = w * a.tau * (o.mass * o.B - (qt > 0.0f ? qt / r.s : 0.0f));
     o.hw = w;
     o.loss = w * a.tau * a.tau * loss;
     return o;
 }
+// what belongs to the class taken, read ahead of its use
+struct Taken { float z, old_lp, adv, ref; };
+template <typename ZT, int KIND>
+__device__ __forceinline__ Taken taken_row(const SoftArgs &a, const RowAt<ZT> &at, long long row, int code) {
+    Taken t = {to_f(at.z[code]), 0.0f, 0.0f, 0.0f};
+    if (KIND == ROW_POLICY) {
+        const long long i = row * a.p_stride;
+        t.old_lp = a.old_lp[i]; t.adv = a.adv[i];
+        if (a.ref) t.ref = a.ref[i];
+    }
+    return t;
+}
 template <int KIND>
-__device__ __forceinline__ RowOut class_row(const SoftArgs &a, Soft r, float za, long long row, float w) {
+__device__ __forceinline__ RowOut class_row(const SoftArgs &a, Soft r, float shift, const Taken &t, float w) {
     RowOut o;
-    o.m = base_of(r.m);
+    o.M = base_of(r.m, a.c);
+    o.shift = shift;
     o.B = 1.0f / r.s;
-    o.lp = (za - r.m) * a.inv_tau - logf(r.s);
+    o.lp = LN2 * (fmaf(t.z - shift, a.c, -o.M) - log2f(r.s));
     o.mass = 0.0f;
     o.loss = 0.0f;
     if (KIND == ROW_POLICY) {
-        const long long i = row * a.p_stride;
-        const RowLoss l = policy_row(o.lp, a.old_lp[i], a.adv[i], a.ref, i, a.lo, a.hi, a.beta);
+        const RowLoss l = policy_row(o.lp, t.old_lp, t.adv, a.ref != nullptr, t.ref, a.lo, a.hi, a.beta);
         o.loss = w * l.loss;
         o.mass = w * l.d * a.inv_tau;
     }
     o.A = -o.mass * o.B;
+    o.special = -o.mass * expm1f(o.lp); // 1 - p, also where p is close to 1
     o.hw = w * a.inv_tau * a.inv_tau;
     return o;
 }
-// A thread's part of the gradient (and hessian); `scale`: of its terms, where it holds terms
-template <typename ZT, int KIND, int V>
-__device__ __forceinline__ void give(const SoftArgs &a, const RowAt<ZT> &at, const RowOut &o, const uint4 (&r)[V], int t, int nt, float scale, int code) {
-    constexpr int E = Pack<ZT>::E, H = E / 2;
-    constexpr bool terms = E == 4 && KIND != ROW_COEF;
-    const float A = o.A * scale, B = o.B * scale;
-    const f2 c2 = pair(a.c, a.c), b2 = pair(-o.m, -o.m), A2 = pair(A, A);
+// the second pass over a row of a preference; y of stat is negative for a row that is far away
+__device__ __forceinline__ RowOut coef_row(const SoftArgs &a, float2 st, float lp, float w) {
+    RowOut o = {};
+    o.shift = st.y < 0.0f ? st.x : 0.0f;
+    o.M = st.y < 0.0f ? 0.0f : base_of(st.x, a.c);
+    o.B = fabsf(st.y); o.lp = lp; o.mass = w; o.A = -w * o.B;
+    o.special = -w * expm1f(o.lp);
+    return o;
+}
+// A thread's part of the gradient (and hessian); terms(i, x): the terms of its granule i, to be multiplied by `scale`
+template <typename ZT, int KIND, int V, typename F>
+__device__ __forceinline__ void give(const SoftArgs &a, const RowAt<ZT> &at, const RowOut &o, int t, int nt, float scale, int code, F terms) {
+    constexpr int E = Pack<ZT>::E;
+    const float A = o.A * scale, B = o.B * scale, c = a.c, nb = -o.M;
     const int special = KIND == ROW_DISTILL ? -1 : code + at.off;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int v = at.vs + t + i * nt;
         if (v >= at.ve) break;
-        f2 x[H], y[H];
-        Pack<ZT>::get(r[i], x);
+        float x[E], y[E];
+        terms(i, x);
 #pragma unroll
-        for (int e = 0; e < H; ++e) {
-            if (!terms) x[e] = ex2_2(mul2(add2(x[e], b2), c2));
-            y[e] = mul2(x[e], A2);
-        }
+        for (int e = 0; e < E; ++e) y[e] = x[e] * A;
         if (at.g) {
             at.store(at.g, v, y);
-            if (KIND != ROW_DISTILL && (unsigned)(special - v * E) < (unsigned)E) at.g[code] = from_f<ZT>(-o.mass * expm1f(o.lp)); // 1 - p, also where p is close to 1
+            if (KIND != ROW_DISTILL && (unsigned)(special - v * E) < (unsigned)E) at.g[code] = from_f<ZT>(o.special);
         }
         if (at.h) {
-            const f2 B2 = pair(B, B), w2 = pair(o.hw, o.hw), minus = pair(-1.0f, -1.0f), one = pair(1.0f, 1.0f);
 #pragma unroll
-            for (int e = 0; e < H; ++e) { const f2 p = mul2(x[e], B2); y[e] = mul2(mul2(p, w2), add2(one, mul2(p, minus))); }
+            for (int e = 0; e < E; ++e) { const float p = x[e] * B; y[e] = o.hw * p * (1.0f - p); }
             at.store(at.h, v, y);
         }
     }
     for (int j = t; j < at.ends; j += nt) {
         const int k = at.end_at(j);
-        const float e = ex2((to_f(at.z[k]) - o.m) * a.c), p = e * o.B;
-        if (at.g) at.g[k] = from_f<ZT>(KIND != ROW_DISTILL && k == code ? -o.mass * expm1f(o.lp) : e * o.A);
+        const float e = ex2(fmaf(to_f(at.z[k]) - o.shift, c, nb)), p = e * o.B;
+        if (at.g) at.g[k] = from_f<ZT>(KIND != ROW_DISTILL && k == code ? o.special : e * o.A);
         if (at.h) at.h[k] = from_f<ZT>(o.hw * p * (1.0f - p));
     }
+}
+// of a part that is held in granules, as predictions or (32 bits, unless it was not summed) as terms
+template <typename ZT, int KIND, int V>
+__device__ __forceinline__ void give(const SoftArgs &a, const RowAt<ZT> &at, const RowOut &o, const uint4 (&r)[V], int t, int nt, float scale, int code) {
+    constexpr int E = Pack<ZT>::E;
+    give<ZT, KIND, V>(a, at, o, t, nt, scale, code, [&](int i, float (&x)[E]) {
+        Pack<ZT>::get(r[i], x);
+        if (E == 8 || KIND == ROW_COEF) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = ex2(fmaf(x[e], a.c, -o.M));
+        }
+    });
 }
 // the named classes, after all others have been written
 template <typename ZT>
@@ -417,19 +536,23 @@ __device__ __forceinline__ void put_slot(const SoftArgs &a, const RowAt<ZT> &at,
 }
 
 enum { SLOT_SOME = 1, SLOT_BAD = 2, SLOT_TWICE = 4 };
-// Slot j of a row into shared memory; those classes among granules v0 .. v1 - 1 are marked in `bits` (bit: element from the first of granule v0)
+// Slot j of a row into shared memory, its prediction z given; those classes among granules v0 .. v1 - 1 are marked in `bits` (bit: element from
+// the first of granule v0)
 template <typename ZT>
-__device__ __forceinline__ int put_into(const SoftArgs &a, const RowAt<ZT> &at, const Slots &s, uint32_t *bits, long long row, int j) {
-    const uint32_t id = a.ids[row * a.ldt + j];
-    const float t = load_t(a.t, a.t_dtype, row * a.ldt + j);
+__device__ __forceinline__ int put_slot_into(const SoftArgs &a, const RowAt<ZT> &at, const Slots &s, uint32_t *bits, int j, uint32_t id, float t, float z) {
     const bool use = id != 0u && t != -INFINITY, ok = use && id <= (uint32_t)a.K;
     s.id[j] = ok ? (int)id - 1 : -1;
     s.t[j] = t;
-    s.z[j] = ok ? to_f(at.z[id - 1]) : 0.0f;
+    s.z[j] = z;
     int flags = (use ? SLOT_SOME : 0) | (use && !ok ? SLOT_BAD : 0);
     const int b = (int)id - 1 + at.off - at.v0 * RowAt<ZT>::E;
     if (ok && b >= 0 && b < (at.v1 - at.v0) * RowAt<ZT>::E && (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1u)) flags |= SLOT_TWICE;
     return flags;
+}
+template <typename ZT>
+__device__ __forceinline__ int put_into(const SoftArgs &a, const RowAt<ZT> &at, const Slots &s, uint32_t *bits, long long row, int j) {
+    const uint32_t id = a.ids[row * a.ldt + j];
+    return put_slot_into(a, at, s, bits, j, id, load_t(a.t, a.t_dtype, row * a.ldt + j), id != 0u && id <= (uint32_t)a.K ? to_f(at.z[id - 1]) : 0.0f);
 }
 
 // Rows of up to V granules for each of G lanes (a power of two up to 32): 32 / G rows a warp, 8 warps a CTA.
@@ -463,7 +586,7 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
     } else if (live && id > (uint32_t)a.K) flags = SLOT_BAD;
     const bool whole = live && !(flags & SLOT_BAD);
     const int code = whole && KIND != ROW_DISTILL ? (int)id - 1 : -1;
-    const float za = code >= 0 ? to_f(at.z[code]) : 0.0f;
+    const Taken taken = code >= 0 ? taken_row<ZT, KIND>(a, at, row, code) : Taken{};
     if (there && !whole) {
         const float value = live ? NAN : 0.0f;
         if (KIND != ROW_LOGP) at.fill(lane, G, value);
@@ -474,25 +597,32 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
         }
     }
     Soft mine_r = {0.0f, 1.0f}, all = mine_r;
+    float shift = 0.0f;
     RowOut o = {};
     if (KIND == ROW_COEF) {
         if (whole) {
-            const float2 st = a.stat[row];
-            o.m = base_of(st.x); o.B = st.y; o.lp = a.logp[row]; o.mass = w; o.A = -w * st.y;
+            o = coef_row(a, a.stat[row], a.logp[row], w);
+            if (o.shift != 0.0f) less<ZT, V>(r, at, o.shift, nullptr, lane, G);
         }
     } else {
-        mine_r = take<ZT, V>(r, at, a.c, KIND == ROW_DISTILL && a.tail && whole ? bits : nullptr, lane, G, whole);
+        const uint32_t *out = KIND == ROW_DISTILL && a.tail && whole ? bits : nullptr;
+        mine_r = take<ZT, V>(r, at, a.c, out, lane, G, whole);
         all = lanes_join(mine_r, a.c, G);
-        if (KIND == ROW_DISTILL) { if (!whole) for (int j = lane; j < a.T; j += G) s.id[j] = -1; __syncwarp(); o = slots_row(a, s, all, flags & SLOT_TWICE, w, lane, G, true); }
-        else if (whole) o = class_row<KIND>(a, all, za, row, w);
+        const bool far = whole && is_far(all.m, a.c) && all.m != INFINITY;
+        if (__any_sync(FULL, far)) {
+            if (far) { shift = all.m; mine_r = {0.0f, take_far<ZT, V>(r, at, shift, a.c, out, lane, G)}; }
+            all = lanes_join(mine_r, a.c, G);
+        }
+        if (KIND == ROW_DISTILL) { if (!whole) for (int j = lane; j < a.T; j += G) s.id[j] = -1; __syncwarp(); o = slots_row(a, s, all, shift, flags & SLOT_TWICE, w, lane, G, true); }
+        else if (whole) o = class_row<KIND>(a, all, shift, taken, w);
     }
     if (whole) {
         if (lane == 0) {
             if ((KIND == ROW_DISTILL || KIND == ROW_POLICY) && a.loss) a.loss[row] = o.loss;
             if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = o.lp;
-            if (KIND == ROW_LOGP) a.stat[row] = make_float2(all.m, o.B);
+            if (KIND == ROW_LOGP) a.stat[row] = shift != 0.0f ? make_float2(shift, -o.B) : make_float2(all.m, o.B);
         }
-        const float scale = E == 4 && KIND != ROW_COEF ? ex2((mine_r.m - o.m) * a.c) : 1.0f;
+        const float scale = E == 4 && KIND != ROW_COEF ? ex2(rise(mine_r.m, a.c, o.M)) : 1.0f;
         if (KIND != ROW_LOGP) give<ZT, KIND, V>(a, at, o, r, lane, G, scale, code);
     }
     if (KIND == ROW_DISTILL) {
@@ -501,110 +631,222 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
     }
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ float2 cluster_read(const float2 *p, int rank) {
-    uint32_t at;
-    float2 v;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
-    return v;
+// What the CTAs of a cluster tell one another: maximum, sum and flags of their parts of a row.  Each writes its words into the shared memory
+// of all; a barrier there counts the bytes.
+struct Mail {
+    uint4 word[8];
+    unsigned long long bar;
+};
+__device__ __forceinline__ uint32_t smem_at(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(unsigned long long *bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_at(bar)), "r"(count) : "memory"); }
+__device__ __forceinline__ void bar_expect(unsigned long long *bar, int bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(unsigned long long *bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_at(bar)) : "memory"); }
+__device__ __forceinline__ void mail_send(Mail *m, int from, int to, Soft r, int flags) {
+    uint32_t at, bar;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_at(&m->word[from])), "r"(to));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_at(&m->bar)), "r"(to));
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at), "r"(__float_as_uint(r.m)),
+                 "r"(__float_as_uint(r.s)), "r"(flags), "r"(0), "r"(bar) : "memory");
+}
+// false: it did not come within some tenths of a second at least
+__device__ __forceinline__ bool bar_wait(unsigned long long *bar, unsigned parity) {
+    for (int k = 0; k < (1 << 20); ++k) {
+        uint32_t done;
+        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                     : "=r"(done) : "r"(smem_at(bar)), "r"(parity) : "memory");
+        if (done) return true;
+    }
+    return false;
 }
 
-__device__ __forceinline__ int cluster_read(const int *p, int rank) {
-    uint32_t at;
-    int v;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-    return v;
-}
-
-// One row for a CTA, or for a cluster of CS CTAs, up to V granules a thread.
-template <typename ZT, int KIND, int V>
-__global__ void __launch_bounds__(V > 4 ? 512 : 1024, V > 4 ? 2 : 1) k_row_ctas(SoftArgs a, int CS, int words) {
+// One row for a CTA of NT threads, or for a cluster of 1 << lcs of them, up to V granules a thread.
+template <typename ZT, int KIND, int V, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs, int words) {
     extern __shared__ __align__(16) unsigned char s_raw[];
+    __shared__ Mail s_mail[2];
     __shared__ float2 s_part[32];
-    __shared__ float2 s_cta;
+    __shared__ RowOut s_out;
     __shared__ int s_flags;
-    constexpr int E = Pack<ZT>::E;
-    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warps = nt >> 5;
-    const long long row = blockIdx.x / (unsigned)CS;
-    const int rank = CS > 1 ? (int)(blockIdx.x % (unsigned)CS) : 0;
-    const RowAt<ZT> at(a, row, rank, CS);
-    const Slots s(s_raw, KIND == ROW_DISTILL ? a.T : 0);
-    uint32_t *bits = reinterpret_cast<uint32_t *>(s_raw + (size_t)a.T * Slots::BYTES);
-    float w = a.w ? a.w[row * a.w_stride] : 1.0f;
-    if (KIND == ROW_COEF) w = a.coef[row];
+    constexpr int E = Pack<ZT>::E, H = E / 2, WARPS = NT / 32;
+    constexpr bool DIST = KIND == ROW_DISTILL;
+    constexpr bool TERMS = E == 4 && KIND != ROW_COEF; // 32-bit predictions become their terms
+    const int t = threadIdx.x, lane = t & 31, CS = 1 << lcs;
+    const long long row = blockIdx.x >> lcs;
+    const int rank = blockIdx.x & (CS - 1);
     uint32_t id = 0u;
-    if (KIND != ROW_DISTILL) id = a.code[row * a.p_stride];
-    bool live = w != 0.0f && (KIND == ROW_DISTILL || id != 0u);
-    uint4 r[V];
-    fetch<ZT, V>(r, at, tid, nt, live);
-    int flags = live && KIND != ROW_DISTILL && id > (uint32_t)a.K ? SLOT_BAD : 0;
-    if (KIND == ROW_DISTILL && live) {
-        if (tid == 0) s_flags = 0;
-        for (int i = tid; i < words; i += nt) bits[i] = 0u;
+    if (!DIST) id = a.code[row * a.p_stride];
+    float w = KIND == ROW_COEF ? a.coef[row] : a.w ? a.w[row * a.w_stride] : 1.0f;
+    if (CS > 1 && KIND != ROW_COEF) {
+        if (t == 0) {
+            for (int q = 0; q < 2; ++q) { bar_init(&s_mail[q].bar, 1); bar_expect(&s_mail[q].bar, 16 * CS); }
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
         __syncthreads();
-        for (int j = tid; j < a.T; j += nt) flags |= put_into(a, at, s, bits, row, j);
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    }
+    const RowAt<ZT> at(a, row, rank, CS);
+    const int left = at.ve - at.vs - t;            // of this thread's granules and those behind them
+    const bool full = at.ve - at.vs >= (V - 1) * NT; // all but the last are there for every thread
+    const int end = t < at.ends ? at.end_at(t) : -1; // fewer than 16: one a thread at most
+    const Slots s(s_raw, DIST ? a.T : 0);
+    uint32_t *bits = reinterpret_cast<uint32_t *>(s_raw + (size_t)a.T * Slots::BYTES);
+    bool live = w != 0.0f && (DIST || id != 0u);
+    uint4 r[V];
+    ZT end_raw = from_f<ZT>(-INFINITY);
+    {
+        const uint4 *p = at.granules() + at.vs + t;
+        const uint4 none = make_uint4(Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE);
+        if (live && full) {
+#pragma unroll
+            for (int i = 0; i < V - 1; ++i) r[i] = __ldg(p + i * NT);
+            r[V - 1] = (V - 1) * NT < left ? __ldg(p + (V - 1) * NT) : none;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) r[i] = live && i * NT < left ? __ldg(p + i * NT) : none;
+        }
+        if (live && end >= 0) end_raw = at.z[end];
+    }
+    // what the class taken brings along, raw: a conversion here would wait for it
+    const int code = DIST ? -1 : (int)id - 1;
+    int flags = live && !DIST && id > (uint32_t)a.K ? SLOT_BAD : 0;
+    ZT code_raw = from_f<ZT>(0.0f);
+    Taken taken = {};
+    float2 st = make_float2(0.0f, 0.0f);
+    float st_lp = 0.0f;
+    if (KIND == ROW_COEF) { st = a.stat[row]; st_lp = a.logp[row]; }
+    else if (!DIST && live && !flags && t < 32) {
+        code_raw = at.z[code];
+        if (KIND == ROW_POLICY) {
+            const long long i = row * a.p_stride;
+            taken.old_lp = a.old_lp[i]; taken.adv = a.adv[i];
+            if (a.ref) taken.ref = a.ref[i];
+        }
+    }
+    if (DIST && live) {
+        if (t == 0) s_flags = 0;
+        for (int i = t; i < words; i += NT) bits[i] = 0u;
+        __syncthreads();
+        for (int j = t; j < a.T; j += NT) flags |= put_into(a, at, s, bits, row, j);
         flags = __reduce_or_sync(FULL, flags);
         if (lane == 0 && flags) atomicOr(&s_flags, flags);
         __syncthreads();
         flags = s_flags;
         live = flags & SLOT_SOME;
     }
+    if (CS > 1 && KIND != ROW_COEF) asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); // the others' mail is open
     if (!live || (flags & SLOT_BAD)) {
         const float value = live ? NAN : 0.0f;
-        if (KIND != ROW_LOGP) at.fill(tid, nt, value);
-        if (tid == 0 && rank == 0) {
+        if (KIND != ROW_LOGP) at.fill(t, NT, value);
+        if (t == 0 && rank == 0) {
             if (KIND != ROW_COEF && a.loss) a.loss[row] = value;
             if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = value;
             if (KIND == ROW_LOGP) a.stat[row] = make_float2(0.0f, value);
         }
         return;
     }
-    const int code = KIND != ROW_DISTILL ? (int)id - 1 : -1;
-    const float za = code >= 0 ? to_f(at.z[code]) : 0.0f;
-    Soft mine = {0.0f, 1.0f}, all = mine;
-    RowOut o = {};
+    Soft mine = {0.0f, 1.0f};
+    RowOut o;
     if (KIND == ROW_COEF) {
-        const float2 st = a.stat[row];
-        o.m = base_of(st.x); o.B = st.y; o.lp = a.logp[row]; o.mass = w; o.A = -w * st.y;
+        o = coef_row(a, st, st_lp, w);
+        if (o.shift != 0.0f) less<ZT, V>(r, at, o.shift, nullptr, t, NT);
     } else {
-        mine = take<ZT, V>(r, at, a.c, KIND == ROW_DISTILL && a.tail ? bits : nullptr, tid, nt, true);
-        all = lanes_join(mine, a.c, 32);
-        if (lane == 0) s_part[tid >> 5] = make_float2(all.m, all.s);
-        __syncthreads();
-        const float2 p = lane < warps ? s_part[lane] : make_float2(-INFINITY, 0.0f);
-        all = lanes_join(Soft{p.x, p.y}, a.c, 32);
-        if (CS > 1) {
-            if (tid == 0) s_cta = make_float2(all.m, all.s);
-            cluster_arrive();
-            cluster_wait();
-            const float2 q = lane < CS ? cluster_read(&s_cta, lane) : make_float2(-INFINITY, 0.0f);
-            all = lanes_join(Soft{q.x, q.y}, a.c, 32);
-            if (KIND == ROW_DISTILL) flags |= __reduce_or_sync(FULL, lane < CS ? cluster_read(&s_flags, lane) : 0); // each sees its own classes twice
-            cluster_arrive(); // a CTA that has read may let the others go: they wait for it at their end
+        const uint32_t *out = DIST && a.tail ? bits : nullptr;
+        if (out) leave_out<ZT, V>(r, at, out, t, NT);
+        if (out && end >= 0 && marked(out, end + at.off - at.v0 * E)) end_raw = from_f<ZT>(-INFINITY);
+        typename Pack<ZT>::Most most;
+#pragma unroll
+        for (int i = 0; i < V; ++i) most.see(r[i]);
+        const float end_z = to_f(end_raw);
+        mine.m = fmaxf(most.get(), end_z);
+        {
+            const float nb = is_far(mine.m, a.c) ? -INFINITY : -base_of(mine.m, a.c);
+            const f2 c2 = pair(a.c, a.c), b2 = pair(nb, nb);
+            f2 sum[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                f2 x[H];
+                Pack<ZT>::get2(r[i], x);
+#pragma unroll
+                for (int e = 0; e < H; ++e) { x[e] = ex2_2(fma2(x[e], c2, b2)); sum[e & 1] = add2(sum[e & 1], x[e]); }
+                if (TERMS) r[i] = Pack<ZT>::put2(x);
+                else asm volatile("" : "+r"(r[i].x), "+r"(r[i].y), "+r"(r[i].z), "+r"(r[i].w)); // they stay packed: unpacked they would take twice the registers
+            }
+            float lo, hi;
+            split(add2(sum[0], sum[1]), lo, hi);
+            mine.s = lo + hi + ex2(fmaf(end_z, a.c, nb));
         }
-        if (KIND == ROW_DISTILL) o = slots_row(a, s, all, flags & SLOT_TWICE, w, lane, 32, tid < 32);
-        else o = class_row<KIND>(a, all, za, row, w);
-    }
-    if (tid == 0 && rank == 0) {
-        if ((KIND == ROW_DISTILL || KIND == ROW_POLICY) && a.loss) a.loss[row] = o.loss;
-        if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = o.lp;
-        if (KIND == ROW_LOGP) a.stat[row] = make_float2(all.m, o.B);
-    }
-    if (KIND != ROW_LOGP && (at.g || at.h)) {
-        const float scale = E == 4 && KIND != ROW_COEF ? ex2((mine.m - o.m) * a.c) : 1.0f;
-        give<ZT, KIND, V>(a, at, o, r, tid, nt, scale, code);
-        if (KIND == ROW_DISTILL) {
+        // the parts of the threads, the warps and the CTAs are joined, the last two by every warp for itself
+        auto whole_row = [&](Mail *mail) {
+            Soft all = lanes_join(mine, a.c, 32);
+            if (lane == 0) s_part[t >> 5] = make_float2(all.m, all.s);
             __syncthreads();
-            for (int j = tid; j < a.T; j += nt) {
-                const int k = s.id[j], v = (k + at.off) / E;
-                if (k >= 0 && v >= at.v0 && v < at.v1) put_slot(a, at, o, s, j, flags & SLOT_TWICE, w);
+            const float2 p = lane < WARPS ? s_part[lane] : make_float2(-INFINITY, 0.0f);
+            all = lanes_join(Soft{p.x, p.y}, a.c, 32);
+            if (CS > 1) {
+                if (t < CS) mail_send(mail, rank, t, all, flags);
+                const bool came = bar_wait(&mail->bar, 0u);
+                const uint4 q = lane < CS ? mail->word[lane] : make_uint4(0xff800000u, 0u, 0u, 0u);
+                all = lanes_join(Soft{__uint_as_float(q.x), __uint_as_float(q.y)}, a.c, 32);
+                if (DIST) flags |= __reduce_or_sync(FULL, q.z); // each sees its own classes twice
+                if (!came) all.s = NAN;
+            }
+            return all;
+        };
+        Soft all = whole_row(&s_mail[0]);
+        float shift = 0.0f;
+        if (is_far(all.m, a.c) && all.m != INFINITY) { // the same for all threads of the row
+            __syncthreads();
+            shift = all.m;
+            mine = {0.0f, take_far<ZT, V>(r, at, shift, a.c, out, t, NT)};
+            all = whole_row(&s_mail[1]);
+        }
+        if (t < 32) {
+            taken.z = to_f(code_raw);
+            if (DIST) o = slots_row(a, s, all, shift, flags & SLOT_TWICE, w, lane, 32, true);
+            else o = class_row<KIND>(a, all, shift, taken, w);
+            if (t == 0) {
+                s_out = o;
+                if (rank == 0) {
+                    if ((DIST || KIND == ROW_POLICY) && a.loss) a.loss[row] = o.loss;
+                    if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = o.lp;
+                    if (KIND == ROW_LOGP) a.stat[row] = shift != 0.0f ? make_float2(shift, -o.B) : make_float2(all.m, o.B);
+                }
             }
         }
+        if (KIND == ROW_LOGP) return;
+        __syncthreads();
+        o = s_out;
     }
-    if (CS > 1 && KIND != ROW_COEF) cluster_wait();
+    if (!(at.g || at.h)) return;
+    if (full && at.whole && !at.h) {
+        // nothing but the gradient, whole granules
+        const float A = TERMS ? o.A * ex2(rise(mine.m, a.c, o.M)) : o.A;
+        const f2 c2 = pair(a.c, a.c), b2 = pair(-o.M, -o.M), A2 = pair(A, A);
+        uint4 *p = reinterpret_cast<uint4 *>(at.g - at.off) + at.vs + t;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (i == V - 1 && (V - 1) * NT >= left) break;
+            f2 x[H];
+            Pack<ZT>::get2(r[i], x);
+#pragma unroll
+            for (int e = 0; e < H; ++e) x[e] = mul2(TERMS ? x[e] : ex2_2(fma2(x[e], c2, b2)), A2);
+            p[i * NT] = Pack<ZT>::put2(x);
+        }
+        const int k = (code + at.off) / E - at.vs - t; // the class taken, by the thread that has written its granule
+        if (!DIST && k >= 0 && k < at.ve - at.vs && k % NT == 0) at.g[code] = from_f<ZT>(o.special);
+        if (end >= 0) at.g[end] = from_f<ZT>(!DIST && end == code ? o.special : ex2(fmaf(to_f(end_raw) - o.shift, a.c, -o.M)) * o.A);
+    } else {
+        give<ZT, KIND, V>(a, at, o, r, t, NT, TERMS ? ex2(rise(mine.m, a.c, o.M)) : 1.0f, code);
+    }
+    if (DIST) {
+        __syncthreads();
+        for (int j = t; j < a.T; j += NT) {
+            const int k = s.id[j], v = (k + at.off) / E;
+            if (k >= 0 && v >= at.v0 && v < at.v1) put_slot(a, at, o, s, j, flags & SLOT_TWICE, w);
+        }
+    }
 }
 
 // Rows of more granules than a cluster holds: one CTA walks over a row twice.
@@ -647,42 +889,60 @@ __global__ void __launch_bounds__(512) k_row_walk(SoftArgs a, int words) {
         return;
     }
     const int code = KIND != ROW_DISTILL ? (int)id - 1 : -1;
-    const float za = code >= 0 ? to_f(at.z[code]) : 0.0f;
+    const Taken taken = code >= 0 ? taken_row<ZT, KIND>(a, at, row, code) : Taken{};
     RowOut o = {};
+    float shift = 0.0f;
+    RowAt<ZT> piece = at; // 4 granules a thread at a time, the ends with the last
     if (KIND == ROW_COEF) {
-        const float2 st = a.stat[row];
-        o.m = base_of(st.x); o.B = st.y; o.lp = a.logp[row]; o.mass = w; o.A = -w * st.y;
+        o = coef_row(a, a.stat[row], a.logp[row], w);
+        shift = o.shift;
     } else {
+        const uint32_t *out = KIND == ROW_DISTILL && a.tail ? bits : nullptr;
         Soft all = {-INFINITY, 0.0f};
-        RowAt<ZT> piece = at; // 4 granules a thread at a time, the ends with the last
         for (piece.vs = at.vs; piece.vs < at.ve || piece.vs == at.vs; piece.vs += 4 * nt) {
             const bool last = piece.vs + 4 * nt >= at.ve;
             piece.ends = last ? at.ends : 0;
             uint4 r[4];
             fetch<ZT, 4>(r, piece, tid, nt, true);
-            all = join(all, take<ZT, 4>(r, piece, a.c, KIND == ROW_DISTILL && a.tail ? bits : nullptr, tid, nt, true), a.c);
+            all = join(all, take<ZT, 4>(r, piece, a.c, out, tid, nt, true), a.c);
         }
-        all = lanes_join(all, a.c, 32);
-        if (lane == 0) s_part[tid >> 5] = make_float2(all.m, all.s);
-        __syncthreads();
-        const float2 p = lane < warps ? s_part[lane] : make_float2(-INFINITY, 0.0f);
-        all = lanes_join(Soft{p.x, p.y}, a.c, 32);
-        if (KIND == ROW_DISTILL) o = slots_row(a, s, all, flags & SLOT_TWICE, w, lane, 32, tid < 32);
-        else o = class_row<KIND>(a, all, za, row, w);
-        if (KIND == ROW_LOGP && tid == 0) a.stat[row] = make_float2(all.m, o.B);
+        auto whole_row = [&]() {
+            all = lanes_join(all, a.c, 32);
+            if (lane == 0) s_part[tid >> 5] = make_float2(all.m, all.s);
+            __syncthreads();
+            const float2 p = lane < warps ? s_part[lane] : make_float2(-INFINITY, 0.0f);
+            all = lanes_join(Soft{p.x, p.y}, a.c, 32);
+        };
+        whole_row();
+        if (is_far(all.m, a.c) && all.m != INFINITY) {
+            __syncthreads();
+            shift = all.m;
+            all = {0.0f, 0.0f};
+            for (piece.vs = at.vs; piece.vs < at.ve || piece.vs == at.vs; piece.vs += 4 * nt) {
+                piece.ends = piece.vs + 4 * nt >= at.ve ? at.ends : 0;
+                uint4 r[4] = {};
+                all.s += take_far<ZT, 4>(r, piece, shift, a.c, out, tid, nt);
+            }
+            whole_row();
+        }
+        if (KIND == ROW_DISTILL) o = slots_row(a, s, all, shift, flags & SLOT_TWICE, w, lane, 32, tid < 32);
+        else o = class_row<KIND>(a, all, shift, taken, w);
+        if (KIND == ROW_LOGP && tid == 0) a.stat[row] = shift != 0.0f ? make_float2(shift, -o.B) : make_float2(all.m, o.B);
     }
     if (tid == 0) {
         if ((KIND == ROW_DISTILL || KIND == ROW_POLICY) && a.loss) a.loss[row] = o.loss;
         if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = o.lp;
     }
     if (KIND == ROW_LOGP || !(at.g || at.h)) return;
-    RowAt<ZT> piece = at;
     for (piece.vs = at.vs; piece.vs < at.ve || piece.vs == at.vs; piece.vs += 4 * nt) {
         piece.ends = piece.vs + 4 * nt >= at.ve ? at.ends : 0;
         uint4 r[4];
         fetch<ZT, 4>(r, piece, tid, nt, true);
         float scale = 1.0f;
-        if (E == 4 && KIND != ROW_COEF) scale = ex2((take<ZT, 4>(r, piece, a.c, nullptr, tid, nt, false).m - o.m) * a.c);
+        if (E == 4 && KIND != ROW_COEF) { // terms
+            if (shift != 0.0f) take_far<ZT, 4>(r, piece, shift, a.c, nullptr, tid, nt);
+            else scale = ex2(rise(take<ZT, 4>(r, piece, a.c, nullptr, tid, nt, false).m, a.c, o.M));
+        } else if (shift != 0.0f) less<ZT, 4>(r, piece, shift, nullptr, tid, nt);
         give<ZT, KIND, 4>(a, piece, o, r, tid, nt, scale, code);
     }
     if (KIND == ROW_DISTILL) {
@@ -744,21 +1004,18 @@ __global__ void __launch_bounds__(256) k_pairs(PairArgs a) {
     }
 }
 
-template <typename K>
-cudaError_t launch_cluster(K kern, unsigned grid, int threads, int cs, size_t smem, cudaStream_t st, const SoftArgs &a, int words) {
-    if (smem > 47 * 1024) { // with the static part
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
+// What may be resident at a time, asked once for every shape of a kernel
+constexpr int LANES_SMEM = 200 * 1024, WALK_SMEM = 160 * 1024; // the attribute is set to the most a kernel is given: calls of several threads do not undo one another's
+cudaError_t launch_cluster(void (*kern)(SoftArgs, int, int), long long rows, int threads, int lcs, size_t smem, cudaStream_t st, const SoftArgs &a, int words) {
     cudaLaunchConfig_t c = {};
     cudaLaunchAttribute at[1];
-    c.gridDim = dim3(grid); c.blockDim = dim3(threads); c.dynamicSmemBytes = smem; c.stream = st;
-    if (cs > 1) {
+    c.gridDim = dim3((unsigned)(rows << lcs)); c.blockDim = dim3(threads); c.dynamicSmemBytes = smem; c.stream = st;
+    if (lcs > 0) {
         at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = cs; at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        at[0].val.clusterDim.x = 1 << lcs; at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
         c.attrs = at; c.numAttrs = 1;
     }
-    return cudaLaunchKernelEx(&c, kern, a, cs, words);
+    return cudaLaunchKernelEx(&c, kern, a, lcs, words);
 }
 template <typename ZT, int KIND>
 int32_t launch_typed(const SoftArgs &a, int sms, cudaStream_t st) {
@@ -774,31 +1031,36 @@ int32_t launch_typed(const SoftArgs &a, int sms, cudaStream_t st) {
         while (V * G < nvec) V *= 2;
         const int words = words_of(nvec);
         const size_t smem = (size_t)(256 / G) * (slots + words * 4);
-        if (smem <= 200 * 1024) {
+        if (smem <= LANES_SMEM) {
             const unsigned grid = (unsigned)((a.n + 256 / G - 1) / (256 / G));
             auto go = [&](void (*kern)(SoftArgs, int, int)) {
-                const cudaError_t e = smem > 47 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
+                const cudaError_t e = smem > 47 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, LANES_SMEM) : cudaSuccess;
                 return e != cudaSuccess ? e : evb_launch(kern, dim3(grid), dim3(256), smem, st, a, G, words);
             };
             EVB_CUDA(V <= 2 ? go(k_row_lanes<ZT, KIND, 2>) : V == 4 ? go(k_row_lanes<ZT, KIND, 4>) : go(k_row_lanes<ZT, KIND, 8>));
             return EVB_OK;
         }
     }
-    int cs = 1;
-    while (cs < 8 && (nvec + cs - 1) / cs > 512 * 8) cs *= 2;
-    while (cs < 8 && a.n * cs * 2 <= sms && (nvec + cs - 1) / cs > 256) cs *= 2; // few rows: more SMs for each
-    const int per = (nvec + cs - 1) / cs;
-    if (per <= 512 * 8) {
-        const bool small = per <= 1024 * 2 && a.n * cs <= 2 * sms;
-        const int V = small ? 2 : 8, threads = std::max(64, ((per + V - 1) / V + 31) / 32 * 32), words = words_of(per);
-        const size_t smem = slots + words * 4;
-        EVB_CUDA(small ? launch_cluster(k_row_ctas<ZT, KIND, 2>, (unsigned)(a.n * cs), threads, cs, smem, st, a, words)
-                       : launch_cluster(k_row_ctas<ZT, KIND, 8>, (unsigned)(a.n * cs), threads, cs, smem, st, a, words));
+    int lcs = 0;
+    auto per = [&] { return (nvec + (1 << lcs) - 1) >> lcs; };
+    auto go = [&](void (*kern)(SoftArgs, int, int), int threads) {
+        return launch_cluster(kern, a.n, threads, lcs, slots + (size_t)words_of(per()) * 4, st, a, words_of(per()));
+    };
+    while (lcs < 3 && (a.n << (lcs + 1)) <= sms && per() > 256) ++lcs; // few rows: several SMs for each
+    if (per() <= 2048 && (a.n << lcs) <= 2 * sms) {
+        EVB_CUDA(per() <= 512 ? go(k_row_ctas<ZT, KIND, 2, 256>, 256) : go(k_row_ctas<ZT, KIND, 2, 1024>, 1024));
+        return EVB_OK;
+    }
+    lcs = 0;
+    while (lcs < 3 && per() > 256 * 8) ++lcs;
+    if (per() <= 512 * 8 && (a.n << lcs) <= 0x7fffffff) {
+        EVB_CUDA(per() <= 512 ? go(k_row_ctas<ZT, KIND, 8, 64>, 64) : per() <= 1024 ? go(k_row_ctas<ZT, KIND, 8, 128>, 128)
+                 : per() <= 2048 ? go(k_row_ctas<ZT, KIND, 8, 256>, 256) : go(k_row_ctas<ZT, KIND, 8, 512>, 512));
         return EVB_OK;
     }
     const int words = words_of(nvec);
     const size_t smem = slots + words * 4;
-    if (smem > 47 * 1024) EVB_CUDA(cudaFuncSetAttribute(k_row_walk<ZT, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem > 47 * 1024) EVB_CUDA(cudaFuncSetAttribute(k_row_walk<ZT, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, WALK_SMEM));
     EVB_CUDA(evb_launch(k_row_walk<ZT, KIND>, dim3((unsigned)a.n), dim3(512), smem, st, a, words));
     return EVB_OK;
 }

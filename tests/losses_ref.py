@@ -120,7 +120,7 @@ def part(z, tau=1.0):
     f = z.to(F8)
     f = torch.where(torch.isfinite(f), f, torch.zeros((), dtype=F8))
     f = torch.maximum(f, f.max(1, keepdim=True).values - 120.0 * tau)      # below that a probability is zero in 32 bits
-    span = (f.max(1).values - f.min(1).values + f.abs().max(1).values) / tau
+    span = (f.max(1).values - f.min(1).values) / tau
     return U * (4 * span + 4 * (z.shape[1] / 32 + 32) + 64)
 
 

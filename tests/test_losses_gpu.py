@@ -251,6 +251,39 @@ def check_preference(pkg, z, zd, label, seq, ref=None, w=None, beta=0.3, smooth=
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("K", [3, 30, 257, 2500, 20011, 70000, 300001])
+def test_rows_far_away(pkg, K, dtype):
+    """Rows whose largest prediction is the type's lowest value, or far from zero: what counts is the distance to it."""
+    rng = np.random.default_rng(K)
+    dt = DTYPES[dtype]
+    low = torch.finfo(dt).min
+    z = torch.full((5, K), low, dtype=dt)                       # row 0: nothing but masks
+    z[1, : K // 2 + 1] = NINF
+    z[2] = low / 2
+    z[2, 0] = z[2, K - 1] = low / 4                             # two classes are far above the others
+    z[3] = torch.from_numpy(rng.normal(size=K).astype(np.float32)).to(dt) + (1000.0 if dtype == "f16" else 3.0e4)
+    z[4, K - 1] = -low                                          # and one is far above zero
+    a = torch.tensor([1, K, K, 2, K], dtype=torch.int32)
+    old, adv = torch.tensor([-np.log(K), -1.0, -0.5, -8.0, -0.1], dtype=torch.float32), torch.ones(5)
+    for tau in (1.0, 1e-3):
+        out = pkg.policy_grads(z.cuda(), a.cuda(), old.cuda(), adv.cuda(), tau=tau, clip=(1.0, 3.0e38), hess=True)
+        loss, logp, grad, h, scale = R.policy(z, a, old, adv, None, None, tau, (1.0, 3.0e38))
+        rel = R.part(z, tau) + 4 * R.U * logp.abs().nan_to_num()
+        R.close(out[1], logp, rel + R.U * logp.abs(), "logp")
+        R.close(out[2], grad, R.rounded(grad, dt, 4 * rel[:, None], 2 * (scale / tau)[:, None]), "grad")
+        h = torch.where(h > torch.finfo(dt).max * (1 + torch.finfo(dt).eps / 4), torch.full_like(h, float("inf")), h)      # more than half a step beyond the type's largest number
+        R.close(out[3], h, R.rounded(h, dt, 4 * rel[:, None], 2 / tau ** 2), "hess")
+    ids = torch.tensor([[1, 2], [K, K - 1], [1, K], [3, 1], [K, 0]], dtype=torch.int32)
+    t = torch.zeros((5, 2))
+    check_distill(pkg.distill_grads(z[[0, 2, 3]].cuda(), ids[[0, 2, 3]].cuda(), t[[0, 2, 3]].cuda(), hess=True), z[[0, 2, 3]], ids[[0, 2, 3]], t[[0, 2, 3]], None,
+                  1.0, False, True)
+    one = pkg.preference_grads(z.cuda(), a.cuda(), torch.tensor([0, 1, 3], dtype=torch.int32).cuda())
+    want = R.preference(z[:3], a[:3], torch.tensor([0, 1, 3]))
+    R.close(one[2][:3], want[2], R.part(z[:3]) + R.U * want[2].abs(), "logp")
+    R.close(one[3][:3], want[3], R.rounded(want[3], dt, 4 * R.part(z[:3])[:, None], 0.2), "grad")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("K", [k for k in CLASSES if k > 1])
 def test_preference_sizes(pkg, K, dtype):
     rng = np.random.default_rng(K + 2)
