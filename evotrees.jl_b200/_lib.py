@@ -87,5 +87,17 @@ def check(rc: int) -> None:
         raise EvbError(rc, lib().evb_last_error().decode("utf-8", "replace"))
 
 
+_raw_stream = None
+
+
+def raw_stream(index: int) -> int:
+    """Address of torch's current stream on a device, without the object around it where torch offers that."""
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return _raw_stream(index)
+
+
 def ptr(a):
     return None if a is None else a.ctypes.data_as(C.c_void_p)

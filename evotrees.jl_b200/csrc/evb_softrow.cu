@@ -189,7 +189,8 @@ template <typename ZT> struct RowAt {
     ZT *g, *h;
     int K, off, v0, v1, vs, ve, head, ends;
     bool whole; // whole granules of g and h can be written: they begin where those of z do
-    __device__ __forceinline__ RowAt(const SoftArgs &a, long long row, int rank, int CS) {
+    // `most` whole granules at most: what is left over goes with the ends
+    __device__ __forceinline__ RowAt(const SoftArgs &a, long long row, int rank, int CS, int most) {
         z = static_cast<const ZT *>(a.z) + row * a.ldz;
         g = a.g ? static_cast<ZT *>(a.g) + row * a.ldg : nullptr;
         h = a.h ? static_cast<ZT *>(a.h) + row * a.ldh : nullptr;
@@ -200,9 +201,8 @@ template <typename ZT> struct RowAt {
         v1 = min(v0 + per, nvec);
         head = v0 == 0 && off > 0 ? min(K, E - off) : 0;
         vs = v0 + (head > 0);
-        const bool tail = v1 == nvec && v1 > vs && (K + off) % E != 0;
-        ve = v1 - tail;
-        ends = head + (tail ? K - (ve * E - off) : 0);
+        ve = min(max(vs, v1 - (v1 == nvec && (K + off) % E != 0)), vs + most);
+        ends = head + max(0, min(K, v1 * E - off) - (ve * E - off));
         whole = (((g ? (uintptr_t)g ^ (uintptr_t)z : 0) | (h ? (uintptr_t)h ^ (uintptr_t)z : 0)) & 15) == 0;
     }
     __device__ __forceinline__ int end_at(int j) const { return j < head ? j : ve * E - off + j - head; } // element of end j
@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
     const long long row0 = (long long)blockIdx.x * (256 / G) + group;
     const bool there = row0 < a.n;
     const long long row = there ? row0 : a.n - 1;
-    const RowAt<ZT> at(a, row, 0, 1);
+    const RowAt<ZT> at(a, row, 0, 1, 0x7fffffff - (1 << 22));
     unsigned char *mine = s_raw + (size_t)group * (KIND == ROW_DISTILL ? a.T * Slots::BYTES + words * 4 : 0);
     const Slots s(mine, KIND == ROW_DISTILL ? a.T : 0);
     uint32_t *bits = reinterpret_cast<uint32_t *>(mine + (size_t)a.T * Slots::BYTES);
@@ -642,7 +642,6 @@ __device__ __forceinline__ void bar_init(unsigned long long *bar, int count) { a
 __device__ __forceinline__ void bar_expect(unsigned long long *bar, int bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(bar)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void bar_arrive(unsigned long long *bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_at(bar)) : "memory"); }
 __device__ __forceinline__ void mail_send(Mail *m, int from, int to, Soft r, int flags) {
     uint32_t at, bar;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_at(&m->word[from])), "r"(to));
@@ -650,12 +649,12 @@ __device__ __forceinline__ void mail_send(Mail *m, int from, int to, Soft r, int
     asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at), "r"(__float_as_uint(r.m)),
                  "r"(__float_as_uint(r.s)), "r"(flags), "r"(0), "r"(bar) : "memory");
 }
-// false: it did not come within some tenths of a second at least
+// waits for a phase of a barrier, about a microsecond a try; false: it did not come within a second
 __device__ __forceinline__ bool bar_wait(unsigned long long *bar, unsigned parity) {
     for (int k = 0; k < (1 << 20); ++k) {
         uint32_t done;
-        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                     : "=r"(done) : "r"(smem_at(bar)), "r"(parity) : "memory");
+        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+                     : "=r"(done) : "r"(smem_at(bar)), "r"(parity), "r"(1000u) : "memory");
         if (done) return true;
     }
     return false;
@@ -686,10 +685,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
         __syncthreads();
         asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     }
-    const RowAt<ZT> at(a, row, rank, CS);
-    const int left = at.ve - at.vs - t;            // of this thread's granules and those behind them
-    const bool full = at.ve - at.vs >= (V - 1) * NT; // all but the last are there for every thread
-    const int end = t < at.ends ? at.end_at(t) : -1; // fewer than 16: one a thread at most
+    const RowAt<ZT> at(a, row, rank, CS, V * NT);
+    const int count = at.ve - at.vs, left = count - t; // whole granules; of them, this thread's and those behind them
+    const int end = t < at.ends ? at.end_at(t) : -1; // as many as threads at most
     const Slots s(s_raw, DIST ? a.T : 0);
     uint32_t *bits = reinterpret_cast<uint32_t *>(s_raw + (size_t)a.T * Slots::BYTES);
     bool live = w != 0.0f && (DIST || id != 0u);
@@ -698,13 +696,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
     {
         const uint4 *p = at.granules() + at.vs + t;
         const uint4 none = make_uint4(Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE, Pack<ZT>::NONE);
-        if (live && full) {
 #pragma unroll
-            for (int i = 0; i < V - 1; ++i) r[i] = __ldg(p + i * NT);
-            r[V - 1] = (V - 1) * NT < left ? __ldg(p + (V - 1) * NT) : none;
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) r[i] = live && i * NT < left ? __ldg(p + i * NT) : none;
+        for (int i = 0; i < V; ++i) {
+            r[i] = none;
+            if (live && i * NT < left) r[i] = __ldg(p + i * NT);
         }
         if (live && end >= 0) end_raw = at.z[end];
     }
@@ -757,7 +752,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
         if (out && end >= 0 && marked(out, end + at.off - at.v0 * E)) end_raw = from_f<ZT>(-INFINITY);
         typename Pack<ZT>::Most most;
 #pragma unroll
-        for (int i = 0; i < V; ++i) most.see(r[i]);
+        for (int i = 0; i < V; ++i) if (i * NT < count) most.see(r[i]);
         const float end_z = to_f(end_raw);
         mine.m = fmaxf(most.get(), end_z);
         {
@@ -766,6 +761,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
             f2 sum[2] = {0, 0};
 #pragma unroll
             for (int i = 0; i < V; ++i) {
+                if (i * NT >= count) break; // the same for all threads
                 f2 x[H];
                 Pack<ZT>::get2(r[i], x);
 #pragma unroll
@@ -820,14 +816,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
         o = s_out;
     }
     if (!(at.g || at.h)) return;
-    if (full && at.whole && !at.h) {
+    if (at.whole && !at.h) {
         // nothing but the gradient, whole granules
         const float A = TERMS ? o.A * ex2(rise(mine.m, a.c, o.M)) : o.A;
         const f2 c2 = pair(a.c, a.c), b2 = pair(-o.M, -o.M), A2 = pair(A, A);
         uint4 *p = reinterpret_cast<uint4 *>(at.g - at.off) + at.vs + t;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            if (i == V - 1 && (V - 1) * NT >= left) break;
+            if (i * NT >= count) break;
+            if (i * NT >= left) continue;
             f2 x[H];
             Pack<ZT>::get2(r[i], x);
 #pragma unroll
@@ -835,7 +832,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
             p[i * NT] = Pack<ZT>::put2(x);
         }
         const int k = (code + at.off) / E - at.vs - t; // the class taken, by the thread that has written its granule
-        if (!DIST && k >= 0 && k < at.ve - at.vs && k % NT == 0) at.g[code] = from_f<ZT>(o.special);
+        if (!DIST && k >= 0 && k < left && k % NT == 0) at.g[code] = from_f<ZT>(o.special);
         if (end >= 0) at.g[end] = from_f<ZT>(!DIST && end == code ? o.special : ex2(fmaf(to_f(end_raw) - o.shift, a.c, -o.M)) * o.A);
     } else {
         give<ZT, KIND, V>(a, at, o, r, t, NT, TERMS ? ex2(rise(mine.m, a.c, o.M)) : 1.0f, code);
@@ -858,7 +855,7 @@ __global__ void __launch_bounds__(512) k_row_walk(SoftArgs a, int words) {
     constexpr int E = Pack<ZT>::E;
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warps = nt >> 5;
     const long long row = blockIdx.x;
-    const RowAt<ZT> at(a, row, 0, 1);
+    const RowAt<ZT> at(a, row, 0, 1, 0x7fffffff - (1 << 22));
     const Slots s(s_raw, KIND == ROW_DISTILL ? a.T : 0);
     uint32_t *bits = reinterpret_cast<uint32_t *>(s_raw + (size_t)a.T * Slots::BYTES);
     float w = a.w ? a.w[row * a.w_stride] : 1.0f;
@@ -1043,19 +1040,20 @@ int32_t launch_typed(const SoftArgs &a, int sms, cudaStream_t st) {
     }
     int lcs = 0;
     auto per = [&] { return (nvec + (1 << lcs) - 1) >> lcs; };
+    auto holds = [&](int threads, int V) { return per() <= threads * V + (threads - 2 * E) / E; }; // the last few as ends, an element a thread
     auto go = [&](void (*kern)(SoftArgs, int, int), int threads) {
         return launch_cluster(kern, a.n, threads, lcs, slots + (size_t)words_of(per()) * 4, st, a, words_of(per()));
     };
     while (lcs < 3 && (a.n << (lcs + 1)) <= sms && per() > 256) ++lcs; // few rows: several SMs for each
-    if (per() <= 2048 && (a.n << lcs) <= 2 * sms) {
-        EVB_CUDA(per() <= 512 ? go(k_row_ctas<ZT, KIND, 2, 256>, 256) : go(k_row_ctas<ZT, KIND, 2, 1024>, 1024));
+    if (holds(1024, 2) && (a.n << lcs) <= 2 * sms) {
+        EVB_CUDA(holds(256, 2) ? go(k_row_ctas<ZT, KIND, 2, 256>, 256) : go(k_row_ctas<ZT, KIND, 2, 1024>, 1024));
         return EVB_OK;
     }
     lcs = 0;
-    while (lcs < 3 && per() > 256 * 8) ++lcs;
-    if (per() <= 512 * 8 && (a.n << lcs) <= 0x7fffffff) {
-        EVB_CUDA(per() <= 512 ? go(k_row_ctas<ZT, KIND, 8, 64>, 64) : per() <= 1024 ? go(k_row_ctas<ZT, KIND, 8, 128>, 128)
-                 : per() <= 2048 ? go(k_row_ctas<ZT, KIND, 8, 256>, 256) : go(k_row_ctas<ZT, KIND, 8, 512>, 512));
+    while (lcs < 3 && !holds(256, 8)) ++lcs;
+    if (holds(512, 8) && (a.n << lcs) <= 0x7fffffff) {
+        EVB_CUDA(holds(64, 8) ? go(k_row_ctas<ZT, KIND, 8, 64>, 64) : holds(128, 8) ? go(k_row_ctas<ZT, KIND, 8, 128>, 128)
+                 : holds(256, 8) ? go(k_row_ctas<ZT, KIND, 8, 256>, 256) : go(k_row_ctas<ZT, KIND, 8, 512>, 512));
         return EVB_OK;
     }
     const int words = words_of(nvec);
