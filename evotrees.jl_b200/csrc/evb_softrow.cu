@@ -631,6 +631,155 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
     }
 }
 
+// Rows of up to 32 classes: a thread per row, 128 rows a CTA, all that they hold staged through shared memory so that memory is read and written
+// in order.  Rows of shared memory are an odd number of words apart: neighbours fall into different banks.
+constexpr int TILE = 128, TILE_K = 32, TILE_T = 32;
+struct TileGeom { int Kp, Tp; uint32_t by_K, by_T; }; // by_*: (c * by) >> 32 is c / K (c / T) for c < 2^13
+template <typename T, typename F>
+__device__ __forceinline__ void tile_read(const T *src, long long ld, int rows, int W, uint32_t by, F put) { // put(row, column, value)
+    const int n = rows * W;
+    int c0 = 0;
+    if (sizeof(T) == 4 && ld == W && ((uintptr_t)src & 15) == 0) {
+        c0 = n & ~3;
+        for (int c = 4 * threadIdx.x; c < c0; c += 4 * TILE) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src + c));
+            const T *x = reinterpret_cast<const T *>(&v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { const int r = W == 1 ? c + e : __umulhi(c + e, by); put(r, c + e - r * W, x[e]); }
+        }
+    }
+    for (int c = c0 + threadIdx.x; c < n; c += TILE) { const int r = W == 1 ? c : __umulhi(c, by), k = c - r * W; put(r, k, src[r * ld + k]); }
+}
+template <typename T>
+__device__ __forceinline__ void tile_write(T *dst, long long ld, int rows, int W, int Wp, uint32_t by, const float *s) {
+    const int n = rows * W;
+    int c0 = 0;
+    if (sizeof(T) == 4 && ld == W && ((uintptr_t)dst & 15) == 0) {
+        c0 = n & ~3;
+        for (int c = 4 * threadIdx.x; c < c0; c += 4 * TILE) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { const int r = W == 1 ? c + e : __umulhi(c + e, by); x[e] = s[r * Wp + c + e - r * W]; }
+            *reinterpret_cast<float4 *>(dst + c) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+    }
+    for (int c = c0 + threadIdx.x; c < n; c += TILE) { const int r = W == 1 ? c : __umulhi(c, by), k = c - r * W; dst[r * ld + k] = from_f<T>(s[r * Wp + k]); }
+}
+template <typename ZT, int KIND>
+__global__ void __launch_bounds__(TILE) k_row_tile(SoftArgs a, TileGeom ge) {
+    extern __shared__ __align__(16) float s_tile[]; // predictions, then gradients [TILE][Kp]; hessians; slots: five words [TILE][Tp] each
+    constexpr bool DIST = KIND == ROW_DISTILL;
+    const long long row0 = (long long)blockIdx.x * TILE, row = row0 + threadIdx.x;
+    const int K = a.K, Kp = ge.Kp, rows = (int)min((long long)TILE, a.n - row0);
+    float *s_z = s_tile, *s_h = s_z + (a.h ? TILE * Kp : 0), *s_s = s_h + TILE * Kp;
+    const int T = DIST ? a.T : 0;
+    const bool here = (int)threadIdx.x < rows;
+    float w = 0.0f;
+    uint32_t id = 0u;
+    Taken taken = {};
+    float2 st = make_float2(0.0f, 0.0f);
+    float st_lp = 0.0f;
+    if (here) {
+        w = KIND == ROW_COEF ? a.coef[row] : a.w ? a.w[row * a.w_stride] : 1.0f;
+        if (!DIST) id = a.code[row * a.p_stride];
+        if (KIND == ROW_POLICY) {
+            const long long i = row * a.p_stride;
+            taken.old_lp = a.old_lp[i]; taken.adv = a.adv[i];
+            if (a.ref) taken.ref = a.ref[i];
+        }
+        if (KIND == ROW_COEF) { st = a.stat[row]; st_lp = a.logp[row]; }
+    }
+    tile_read(static_cast<const ZT *>(a.z) + row0 * a.ldz, a.ldz, rows, K, ge.by_K, [&](int r, int k, ZT v) { s_z[r * Kp + k] = to_f(v); });
+    if (DIST) {
+        const int Tp = ge.Tp;
+        tile_read(a.ids + row0 * a.ldt, a.ldt, rows, T, ge.by_T, [&](int r, int j, uint32_t v) { reinterpret_cast<uint32_t *>(s_s)[r * Tp + j] = v; });
+        float *s_t = s_s + TILE * Tp;
+        if (a.t_dtype == EVB_F32) tile_read(static_cast<const float *>(a.t) + row0 * a.ldt, a.ldt, rows, T, ge.by_T, [&](int r, int j, float v) { s_t[r * Tp + j] = v; });
+        else if (a.t_dtype == EVB_BF16) tile_read(static_cast<const __nv_bfloat16 *>(a.t) + row0 * a.ldt, a.ldt, rows, T, ge.by_T, [&](int r, int j, __nv_bfloat16 v) { s_t[r * Tp + j] = to_f(v); });
+        else tile_read(static_cast<const __half *>(a.t) + row0 * a.ldt, a.ldt, rows, T, ge.by_T, [&](int r, int j, __half v) { s_t[r * Tp + j] = to_f(v); });
+    }
+    __syncthreads();
+    if (here) {
+        float *z = s_z + threadIdx.x * Kp, *h = s_h + threadIdx.x * Kp;
+        bool live = w != 0.0f && (DIST || id != 0u);
+        int flags = !DIST && live && id > (uint32_t)K ? SLOT_BAD : 0;
+        uint32_t named = 0u; // a bit per class
+        Slots s(s_s, 0);
+        if (DIST) {
+            s.id = reinterpret_cast<int *>(s_s) + threadIdx.x * ge.Tp;
+            s.t = s_s + (TILE + threadIdx.x) * ge.Tp;
+            s.z = s.t + TILE * ge.Tp; s.q = s.z + TILE * ge.Tp; s.lp = s.q + TILE * ge.Tp;
+            for (int j = 0; j < T && live; ++j) {
+                const uint32_t k = (uint32_t)s.id[j];
+                const bool use = k != 0u && s.t[j] != -INFINITY, ok = use && k <= (uint32_t)K;
+                flags |= use ? ok ? SLOT_SOME | (named >> (k - 1) & 1u ? SLOT_TWICE : 0) : SLOT_SOME | SLOT_BAD : 0;
+                s.id[j] = ok ? (int)k - 1 : -1;
+                if (ok) { named |= 1u << (k - 1); s.z[j] = z[k - 1]; }
+            }
+            live = live && (flags & SLOT_SOME);
+        }
+        float loss = 0.0f, lp = 0.0f;
+        float2 stat = make_float2(0.0f, 0.0f);
+        if (!live || (flags & SLOT_BAD)) {
+            loss = lp = stat.y = live ? NAN : 0.0f;
+            for (int k = 0; k < K; ++k) { z[k] = loss; if (a.h) h[k] = loss; }
+        } else {
+            const uint32_t out = DIST && a.tail ? named : 0u;
+            RowOut o = {};
+            float m = -INFINITY;
+            if (KIND == ROW_COEF) {
+                o = coef_row(a, st, st_lp, w);
+                m = st.x;
+            } else {
+                for (int k = 0; k < K; ++k) if (!(out >> k & 1u)) m = fmaxf(m, z[k]);
+            }
+            // 2^(c (z - max)): differences, so that no prediction is too far away
+            const float base = m == -INFINITY ? 0.0f : m;
+            float sum = 0.0f;
+            if (!DIST) taken.z = z[id - 1] - base;
+            for (int k = 0; k < K; ++k) {
+                const float e = ex2((z[k] - base) * a.c);
+                if (!(out >> k & 1u)) sum += e;
+                z[k] = e;
+            }
+            const float zero = m == -INFINITY ? m : 0.0f; // the maximum, less itself
+            if (DIST) { o = slots_row(a, s, Soft{zero, sum}, base, flags & SLOT_TWICE, w, 0, 1, true); loss = o.loss; }
+            else if (KIND != ROW_COEF) {
+                o = class_row<KIND>(a, Soft{zero, sum}, 0.0f, taken, w);
+                loss = o.loss; lp = o.lp;
+                stat = make_float2(m, is_far(m, a.c) ? -o.B : o.B);
+            }
+            if (KIND != ROW_LOGP) {
+                for (int k = 0; k < K; ++k) {
+                    const float e = z[k], p = e * o.B;
+                    z[k] = e * o.A;
+                    if (a.h) h[k] = o.hw * p * (1.0f - p);
+                }
+                if (!DIST) z[id - 1] = o.special;
+                else for (int j = 0; j < T; ++j) {
+                    if (s.id[j] < 0) continue;
+                    float q = s.q[j];
+                    if (flags & SLOT_TWICE) {
+                        if (!first_slot(s, j)) continue;
+                        q = 0.0f;
+                        for (int i = j; i < T; ++i) if (s.id[i] == s.id[j]) q += s.q[i];
+                    }
+                    const float p = expf(s.lp[j]);
+                    z[s.id[j]] = w * a.tau * (o.mass * p - q);
+                    if (a.h) h[s.id[j]] = o.hw * p * (1.0f - p);
+                }
+            }
+        }
+        if (KIND != ROW_COEF && a.loss) a.loss[row] = loss;
+        if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = lp;
+        if (KIND == ROW_LOGP) a.stat[row] = stat;
+    }
+    if (KIND == ROW_LOGP) return;
+    __syncthreads();
+    if (a.g) tile_write(static_cast<ZT *>(a.g) + row0 * a.ldg, a.ldg, rows, K, Kp, ge.by_K, s_z);
+    if (a.h) tile_write(static_cast<ZT *>(a.h) + row0 * a.ldh, a.ldh, rows, K, Kp, ge.by_K, s_h);
+}
+
 // What the CTAs of a cluster tell one another: maximum, sum and flags of their parts of a row.  Each writes its words into the shared memory
 // of all; a barrier there counts the bytes.
 struct Mail {
@@ -1002,7 +1151,7 @@ __global__ void __launch_bounds__(256) k_pairs(PairArgs a) {
 }
 
 // What may be resident at a time, asked once for every shape of a kernel
-constexpr int LANES_SMEM = 200 * 1024, WALK_SMEM = 160 * 1024; // the attribute is set to the most a kernel is given: calls of several threads do not undo one another's
+constexpr int LANES_SMEM = 200 * 1024, WALK_SMEM = 160 * 1024, TILE_SMEM = 128 * 1024; // the attribute is set to the most a kernel is given: calls of several threads do not undo one another's
 cudaError_t launch_cluster(void (*kern)(SoftArgs, int, int), long long rows, int threads, int lcs, size_t smem, cudaStream_t st, const SoftArgs &a, int words) {
     cudaLaunchConfig_t c = {};
     cudaLaunchAttribute at[1];
@@ -1022,6 +1171,16 @@ int32_t launch_typed(const SoftArgs &a, int sms, cudaStream_t st) {
     const int nvec = (a.K + (aligned ? 0 : E - 1) + E - 1) / E;
     const size_t slots = KIND == ROW_DISTILL ? (size_t)a.T * Slots::BYTES : 0;
     auto words_of = [&](int granules) { return KIND == ROW_DISTILL ? (granules * E + 31) / 32 : 0; };
+    if (a.K <= TILE_K && (KIND != ROW_DISTILL || a.T <= TILE_T)) {
+        TileGeom ge;
+        ge.Kp = a.K | 1; ge.Tp = a.T | 1;
+        ge.by_K = (uint32_t)((0x100000000ull + a.K - 1) / a.K); // not used for 1
+        ge.by_T = a.T > 0 ? (uint32_t)((0x100000000ull + a.T - 1) / a.T) : 0u;
+        const size_t smem = 4 * (size_t)TILE * (ge.Kp * (a.h ? 2 : 1) + (KIND == ROW_DISTILL ? 5 * ge.Tp : 0));
+        if (smem > 47 * 1024) EVB_CUDA(cudaFuncSetAttribute(k_row_tile<ZT, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_SMEM));
+        EVB_CUDA(evb_launch(k_row_tile<ZT, KIND>, dim3((unsigned)((a.n + TILE - 1) / TILE)), dim3(TILE), smem, st, a, ge));
+        return EVB_OK;
+    }
     if (nvec <= 256) { // within a warp
         int G = 1, V = 1;
         while (G < 32 && G * 8 < nvec) G *= 2;
