@@ -385,7 +385,7 @@ struct Slots {
         z = t + T; q = z + T; lp = q + T;
     }
 };
-constexpr float LN2 = 0.693147180559945309f;
+constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
 struct RowOut {
     float M, A, B;      // gradient A e and probability B e of the classes that are not named, e = 2^(c (z - shift) - M)
     float shift;        // 0, or the maximum of a row that is far away
@@ -399,8 +399,8 @@ __device__ __forceinline__ bool first_slot(const Slots &s, int j) {
     for (int i = 0; i < j; ++i) if (s.id[i] == s.id[j]) return false;
     return true;
 }
-// r: what the scan found.  `width` lanes share the slots; `keep`: these lanes write q and lp
-__device__ __forceinline__ RowOut slots_row(const SoftArgs &a, const Slots &s, Soft r, float shift, bool dup, float w, int lane, int width, bool keep) {
+// r: what the scan found.  `width` lanes share the slots
+__device__ __forceinline__ RowOut slots_row(const SoftArgs &a, const Slots &s, Soft r, float shift, bool dup, float w, int lane, int width) {
     const float c = a.c;
     float tmax = -INFINITY, zmax = r.m;
     for (int j = lane; j < a.T; j += width) if (s.id[j] >= 0) { tmax = fmaxf(tmax, s.t[j]); zmax = fmaxf(zmax, s.z[j] - shift); }
@@ -410,18 +410,21 @@ __device__ __forceinline__ RowOut slots_row(const SoftArgs &a, const Slots &s, S
     float Q = 0.0f, named = 0.0f;
     for (int j = lane; j < a.T; j += width) {
         if (s.id[j] < 0) continue;
-        Q += a.tail ? expf(s.t[j]) : expf((s.t[j] - tmax) * a.inv_tau);
+        const float e = a.tail ? ex2(s.t[j] * LOG2E) : ex2((s.t[j] - tmax) * c);
+        s.q[j] = e;
+        Q += e;
         if (a.tail && (!dup || first_slot(s, j))) named += ex2(fmaf(s.z[j] - shift, c, -base));
     }
     Q = lanes_sum(Q, width);
     Soft all = r;
     if (a.tail) all = {zmax, lanes_sum(named, width) + r.s * ex2(rise(r.m, c, base))};
-    const float M = base_of(all.m, c), ls = log2f(all.s), lq = logf(Q);
+    const float M = base_of(all.m, c), ls = log2f(all.s), lq = logf(Q), rQ = a.tail ? 1.0f : 1.0f / Q;
     float loss = 0.0f;
     for (int j = lane; j < a.T; j += width) {
         if (s.id[j] < 0) continue;
-        const float lt = a.tail ? s.t[j] : (s.t[j] - tmax) * a.inv_tau - lq, q = expf(lt), lp = LN2 * (fmaf(s.z[j] - shift, c, -M) - ls);
-        if (keep) { s.q[j] = q; s.lp[j] = lp; }
+        const float lt = a.tail ? s.t[j] : (s.t[j] - tmax) * a.inv_tau - lq, q = s.q[j] * rQ, lp = LN2 * (fmaf(s.z[j] - shift, c, -M) - ls);
+        s.q[j] = q;
+        s.lp[j] = lp;
         if (q != 0.0f) loss += q * (lt - lp);
     }
     loss = lanes_sum(loss, width);
@@ -438,6 +441,7 @@ __device__ __forceinline__ RowOut slots_row(const SoftArgs &a, const Slots &s, S
     o.loss = w * a.tau * a.tau * loss;
     return o;
 }
+__device__ __forceinline__ float less_p(float lp) { return lp < -0.5f ? 1.0f - ex2(lp * LOG2E) : -expm1f(lp); } // 1 - p, also where p is close to 1
 // what belongs to the class taken, read ahead of its use
 struct Taken { float z, old_lp, adv, ref; };
 template <typename ZT, int KIND>
@@ -465,7 +469,7 @@ __device__ __forceinline__ RowOut class_row(const SoftArgs &a, Soft r, float shi
         o.mass = w * l.d * a.inv_tau;
     }
     o.A = -o.mass * o.B;
-    o.special = -o.mass * expm1f(o.lp); // 1 - p, also where p is close to 1
+    o.special = o.mass * less_p(o.lp);
     o.hw = w * a.inv_tau * a.inv_tau;
     return o;
 }
@@ -475,7 +479,7 @@ __device__ __forceinline__ RowOut coef_row(const SoftArgs &a, float2 st, float l
     o.shift = st.y < 0.0f ? st.x : 0.0f;
     o.M = st.y < 0.0f ? 0.0f : base_of(st.x, a.c);
     o.B = fabsf(st.y); o.lp = lp; o.mass = w; o.A = -w * o.B;
-    o.special = -w * expm1f(o.lp);
+    o.special = w * less_p(o.lp);
     return o;
 }
 // A thread's part of the gradient (and hessian); terms(i, x): the terms of its granule i, to be multiplied by `scale`
@@ -530,7 +534,7 @@ __device__ __forceinline__ void put_slot(const SoftArgs &a, const RowAt<ZT> &at,
         q = 0.0f;
         for (int i = j; i < a.T; ++i) if (s.id[i] == s.id[j]) q += s.q[i];
     }
-    const float p = expf(s.lp[j]);
+    const float p = ex2(s.lp[j] * LOG2E);
     if (at.g) at.g[s.id[j]] = from_f<ZT>(w * a.tau * (o.mass * p - q));
     if (at.h) at.h[s.id[j]] = from_f<ZT>(o.hw * p * (1.0f - p));
 }
@@ -613,7 +617,7 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
             if (far) { shift = all.m; mine_r = {0.0f, take_far<ZT, V>(r, at, shift, a.c, out, lane, G)}; }
             all = lanes_join(mine_r, a.c, G);
         }
-        if (KIND == ROW_DISTILL) { if (!whole) for (int j = lane; j < a.T; j += G) s.id[j] = -1; __syncwarp(); o = slots_row(a, s, all, shift, flags & SLOT_TWICE, w, lane, G, true); }
+        if (KIND == ROW_DISTILL) { if (!whole) for (int j = lane; j < a.T; j += G) s.id[j] = -1; __syncwarp(); o = slots_row(a, s, all, shift, flags & SLOT_TWICE, w, lane, G); }
         else if (whole) o = class_row<KIND>(a, all, shift, taken, w);
     }
     if (whole) {
@@ -743,7 +747,7 @@ __global__ void __launch_bounds__(TILE) k_row_tile(SoftArgs a, TileGeom ge) {
                 z[k] = e;
             }
             const float zero = m == -INFINITY ? m : 0.0f; // the maximum, less itself
-            if (DIST) { o = slots_row(a, s, Soft{zero, sum}, base, flags & SLOT_TWICE, w, 0, 1, true); loss = o.loss; }
+            if (DIST) { o = slots_row(a, s, Soft{zero, sum}, base, flags & SLOT_TWICE, w, 0, 1); loss = o.loss; }
             else if (KIND != ROW_COEF) {
                 o = class_row<KIND>(a, Soft{zero, sum}, 0.0f, taken, w);
                 loss = o.loss; lp = o.lp;
@@ -764,7 +768,7 @@ __global__ void __launch_bounds__(TILE) k_row_tile(SoftArgs a, TileGeom ge) {
                         q = 0.0f;
                         for (int i = j; i < T; ++i) if (s.id[i] == s.id[j]) q += s.q[i];
                     }
-                    const float p = expf(s.lp[j]);
+                    const float p = ex2(s.lp[j] * LOG2E);
                     z[s.id[j]] = w * a.tau * (o.mass * p - q);
                     if (a.h) h[s.id[j]] = o.hw * p * (1.0f - p);
                 }
@@ -778,6 +782,132 @@ __global__ void __launch_bounds__(TILE) k_row_tile(SoftArgs a, TileGeom ge) {
     __syncthreads();
     if (a.g) tile_write(static_cast<ZT *>(a.g) + row0 * a.ldg, a.ldg, rows, K, Kp, ge.by_K, s_z);
     if (a.h) tile_write(static_cast<ZT *>(a.h) + row0 * a.ldh, a.ldh, rows, K, Kp, ge.by_K, s_h);
+}
+
+// The same for 2 to 8 classes of 32 bits, their number known to the compiler: a row's predictions stay in registers, read by their thread alone (the
+// rows of a warp are neighbours: what one thread leaves of a line, others take); gradients and hessians go out through shared memory.
+template <int KIND, int K>
+__global__ void __launch_bounds__(TILE) k_row_few(SoftArgs a) {
+    extern __shared__ __align__(16) float s_tile[]; // gradients [TILE][K], hessians
+    constexpr bool DIST = KIND == ROW_DISTILL;
+    const long long row0 = (long long)blockIdx.x * TILE, row = row0 + threadIdx.x;
+    const int rows = (int)min((long long)TILE, a.n - row0);
+    float *s_g = s_tile + threadIdx.x * K, *s_h = s_g + TILE * K;
+    if ((int)threadIdx.x < rows) {
+        const float *zp = static_cast<const float *>(a.z) + row * a.ldz;
+        float z[K], y[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) z[k] = __ldg(zp + k);
+        const float w = KIND == ROW_COEF ? a.coef[row] : a.w ? a.w[row * a.w_stride] : 1.0f, c = a.c;
+        const uint32_t id = DIST ? 0u : a.code[row * a.p_stride];
+        Taken taken = {};
+        if (KIND == ROW_POLICY) {
+            const long long i = row * a.p_stride;
+            taken.old_lp = a.old_lp[i]; taken.adv = a.adv[i];
+            if (a.ref) taken.ref = a.ref[i];
+        }
+        // the teacher's probability of every class; the classes that it names
+        float Q = 0.0f, entropy = 0.0f, q[K];
+        uint32_t named = 0u;
+        bool some = false, bad = !DIST && id > (uint32_t)K;
+        if (DIST) {
+            const long long at = row * a.ldt;
+#pragma unroll
+            for (int k = 0; k < K; ++k) q[k] = 0.0f;
+            float tmax = -INFINITY;
+            if (!a.tail) for (int j = 0; j < a.T; ++j) if (a.ids[at + j] != 0u) tmax = fmaxf(tmax, load_t(a.t, a.t_dtype, at + j));
+            for (int j = 0; j < a.T; ++j) {
+                const uint32_t k1 = a.ids[at + j];
+                const float t = load_t(a.t, a.t_dtype, at + j);
+                if (k1 == 0u || t == -INFINITY) continue;
+                some = true;
+                bad = bad || k1 > (uint32_t)K;
+                named |= 1u << ((k1 - 1) & 31);
+                const float lt = a.tail ? t : (t - tmax) * a.inv_tau, e = ex2(lt * LOG2E);
+                Q += e;
+                if (e != 0.0f) entropy += e * lt;
+#pragma unroll
+                for (int k = 0; k < K; ++k) if (k + 1 == (int)k1) q[k] += e;
+            }
+        }
+        const bool live = w != 0.0f && (DIST ? some : id != 0u);
+        float loss = 0.0f, lp = 0.0f;
+        float2 stat = make_float2(0.0f, 0.0f);
+        if (!live || bad) {
+            loss = lp = stat.y = live ? NAN : 0.0f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) y[k] = z[k] = loss;
+        } else {
+            // 2^(c (z - max)): differences, so that no prediction is too far away.  With a tail the classes that are not named have a maximum of their own
+            const uint32_t out = DIST && a.tail ? named : 0u;
+            float m = -INFINITY, all_m = -INFINITY, sum = 0.0f, rest = 0.0f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) { all_m = fmaxf(all_m, z[k]); if (!(out >> k & 1u)) m = fmaxf(m, z[k]); }
+            const float base = all_m == -INFINITY ? 0.0f : all_m;
+#pragma unroll
+            for (int k = 0; k < K; ++k) { y[k] = ex2((z[k] - base) * c); sum += y[k]; }
+            const float zero = all_m == -INFINITY ? all_m : 0.0f;
+            if (DIST) {
+                const float ls = log2f(sum), lq = a.tail ? 0.0f : logf(Q), rQ = a.tail ? 1.0f : 1.0f / Q, r = 1.0f / sum;
+                if (zero != 0.0f) loss = NAN;
+                loss += entropy * rQ - (a.tail ? 0.0f : lq);
+                float qt = 0.0f, rbase = 0.0f, rr = 0.0f;
+                if (a.tail && m != -INFINITY) {
+                    qt = fmaxf(0.0f, 1.0f - Q);
+                    rbase = m;
+#pragma unroll
+                    for (int k = 0; k < K; ++k) if (!(out >> k & 1u)) rest += ex2((z[k] - rbase) * c);
+                    rr = qt / rest;
+                    if (qt > 0.0f) loss += qt * (logf(qt) - LN2 * ((rbase - base) * c + log2f(rest) - ls));
+                }
+                const float mass = a.tail ? Q + qt : 1.0f, f = w * a.tau;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const float qk = q[k] * rQ, p = y[k] * r;
+                    if (qk != 0.0f) loss -= qk * (LN2 * ((z[k] - base) * c - ls));
+                    float g = mass * p - qk;
+                    if (a.tail && !(out >> k & 1u) && qt > 0.0f) g = mass * p - rr * ex2((z[k] - rbase) * c);
+                    z[k] = f * g;
+                    y[k] = w * p * (1.0f - p);
+                }
+                loss *= w * a.tau * a.tau;
+            } else {
+                RowOut o;
+#pragma unroll
+                for (int k = 0; k < K; ++k) if (k + 1 == (int)id) taken.z = z[k] - base;
+                if (KIND == ROW_COEF) o = coef_row(a, a.stat[row], a.logp[row], w);
+                else {
+                    o = class_row<KIND>(a, Soft{zero, sum}, 0.0f, taken, w);
+                    loss = o.loss; lp = o.lp;
+                    stat = make_float2(all_m, is_far(all_m, c) ? -o.B : o.B);
+                }
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const float p = y[k] * o.B;
+                    z[k] = k + 1 == (int)id ? o.special : y[k] * o.A;
+                    y[k] = o.hw * p * (1.0f - p);
+                }
+            }
+        }
+        if (KIND != ROW_COEF && a.loss) a.loss[row] = loss;
+        if ((KIND == ROW_POLICY || KIND == ROW_LOGP) && a.logp) a.logp[row] = lp;
+        if (KIND == ROW_LOGP) a.stat[row] = stat;
+#pragma unroll
+        for (int k = 0; k < K; ++k) { s_g[k] = z[k]; if (a.h) s_h[k] = y[k]; }
+    }
+    if (KIND == ROW_LOGP) return;
+    __syncthreads();
+    auto give = [&](float *dst, long long ld, const float *from) {
+        const int n = rows * K;
+        if (ld == K && ((uintptr_t)dst & 15) == 0) {
+            for (int c = threadIdx.x; c < n >> 2; c += TILE) reinterpret_cast<float4 *>(dst)[c] = reinterpret_cast<const float4 *>(from)[c];
+            for (int c = (n & ~3) + threadIdx.x; c < n; c += TILE) dst[c] = from[c];
+        } else {
+            for (int c = threadIdx.x; c < n; c += TILE) { const int r = c / K; dst[r * ld + (c - r * K)] = from[c]; }
+        }
+    };
+    if (a.g) give(static_cast<float *>(a.g) + row0 * a.ldg, a.ldg, s_tile);
+    if (a.h) give(static_cast<float *>(a.h) + row0 * a.ldh, a.ldh, s_tile + TILE * K);
 }
 
 // What the CTAs of a cluster tell one another: maximum, sum and flags of their parts of a row.  Each writes its words into the shared memory
@@ -949,7 +1079,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
         }
         if (t < 32) {
             taken.z = to_f(code_raw);
-            if (DIST) o = slots_row(a, s, all, shift, flags & SLOT_TWICE, w, lane, 32, true);
+            if (DIST) o = slots_row(a, s, all, shift, flags & SLOT_TWICE, w, lane, 32);
             else o = class_row<KIND>(a, all, shift, taken, w);
             if (t == 0) {
                 s_out = o;
@@ -1000,6 +1130,7 @@ template <typename ZT, int KIND>
 __global__ void __launch_bounds__(512) k_row_walk(SoftArgs a, int words) {
     extern __shared__ __align__(16) unsigned char s_raw[];
     __shared__ float2 s_part[32];
+    __shared__ RowOut s_out;
     __shared__ int s_flags;
     constexpr int E = Pack<ZT>::E;
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warps = nt >> 5;
@@ -1071,8 +1202,14 @@ __global__ void __launch_bounds__(512) k_row_walk(SoftArgs a, int words) {
             }
             whole_row();
         }
-        if (KIND == ROW_DISTILL) o = slots_row(a, s, all, shift, flags & SLOT_TWICE, w, lane, 32, tid < 32);
-        else o = class_row<KIND>(a, all, shift, taken, w);
+        if (KIND == ROW_DISTILL) {
+            if (tid < 32) {
+                o = slots_row(a, s, all, shift, flags & SLOT_TWICE, w, lane, 32);
+                if (tid == 0) s_out = o;
+            }
+            __syncthreads();
+            o = s_out;
+        } else o = class_row<KIND>(a, all, shift, taken, w);
         if (KIND == ROW_LOGP && tid == 0) a.stat[row] = shift != 0.0f ? make_float2(shift, -o.B) : make_float2(all.m, o.B);
     }
     if (tid == 0) {
@@ -1171,6 +1308,22 @@ int32_t launch_typed(const SoftArgs &a, int sms, cudaStream_t st) {
     const int nvec = (a.K + (aligned ? 0 : E - 1) + E - 1) / E;
     const size_t slots = KIND == ROW_DISTILL ? (size_t)a.T * Slots::BYTES : 0;
     auto words_of = [&](int granules) { return KIND == ROW_DISTILL ? (granules * E + 31) / 32 : 0; };
+    if constexpr (E == 4) {
+        if (a.K >= 2 && a.K <= 8) {
+            const size_t smem = 4 * (size_t)TILE * a.K * (a.h ? 2 : 1);
+            auto go = [&](void (*kern)(SoftArgs)) { return evb_launch(kern, dim3((unsigned)((a.n + TILE - 1) / TILE)), dim3(TILE), smem, st, a); };
+            switch (a.K) {
+            case 2: EVB_CUDA(go(k_row_few<KIND, 2>)); break;
+            case 3: EVB_CUDA(go(k_row_few<KIND, 3>)); break;
+            case 4: EVB_CUDA(go(k_row_few<KIND, 4>)); break;
+            case 5: EVB_CUDA(go(k_row_few<KIND, 5>)); break;
+            case 6: EVB_CUDA(go(k_row_few<KIND, 6>)); break;
+            case 7: EVB_CUDA(go(k_row_few<KIND, 7>)); break;
+            default: EVB_CUDA(go(k_row_few<KIND, 8>));
+            }
+            return EVB_OK;
+        }
+    }
     if (a.K <= TILE_K && (KIND != ROW_DISTILL || a.T <= TILE_T)) {
         TileGeom ge;
         ge.Kp = a.K | 1; ge.Tp = a.T | 1;
