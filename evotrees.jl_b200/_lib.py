@@ -16,9 +16,9 @@ LIB_PATH = os.path.join(HERE, "libevotrees_b200.so")
 EVB_F32, EVB_U32, EVB_F64, EVB_BF16, EVB_F16 = 0, 1, 2, 3, 4
 ERR_LIMIT, ERR_STALE = -7, -8
 LOSS_CODES = {"mse": 0, "logloss": 1, "mlogloss": 2, "gaussian_mle": 3, "poisson": 4, "gamma": 5, "tweedie": 6, "logistic_mle": 7,
-              "mae": 8, "cred_var": 9, "cred_std": 10, "quantile": 11, "multiquantile": 12}
+              "mae": 8, "cred_var": 9, "cred_std": 10, "quantile": 11, "multiquantile": 12, "distill": 13, "policy": 14, "preference": 15}
 METRIC_CODES = {"mse": 0, "rmse": 0, "mae": 1, "logloss": 2, "mlogloss": 3, "gaussian_mle": 4, "poisson": 5, "gamma": 6, "tweedie": 7,
-                "logistic_mle": 8, "quantile": 9, "multiquantile": 10}  # rmse = sqrt of the mse sums
+                "logistic_mle": 8, "quantile": 9, "multiquantile": 10, "distill": 11, "policy": 12, "preference": 13}  # rmse = sqrt of the mse sums
 FLAG_TIMING, FLAG_FULL_PARTITION, FLAG_KEEP_ALL_HIST = 1, 2, 4
 NTIMERS = 12
 TIMER_NAMES = ["grads", "rows_init", "hist", "hist_reduce", "allreduce", "scan", "partition", "plan", "finalize",

@@ -122,9 +122,9 @@ static TreeBlockLayout tree_block_layout(int D, int nn, int K) {
 
 static void drop_graphs(evb_handle *h);
 static void free_eval(evb_handle *h) {
-    void *ptrs[] = {h->ev_xT, h->ev_y, h->ev_w, h->ev_pred, h->ev_part};
+    void *ptrs[] = {h->ev_xT, h->ev_y, h->ev_w, h->ev_pred, h->ev_part, h->ev_loss};
     for (void *p : ptrs) evb_dev_free(p);
-    h->ev_xT = nullptr; h->ev_y = nullptr; h->ev_w = nullptr; h->ev_pred = nullptr; h->ev_part = nullptr;
+    h->ev_xT = nullptr; h->ev_y = nullptr; h->ev_w = nullptr; h->ev_pred = nullptr; h->ev_part = nullptr; h->ev_loss = nullptr;
     h->ev_n = 0;
 }
 static void free_handle(evb_handle *h) {
@@ -195,6 +195,8 @@ static int32_t create_impl(evb_handle *h, const evb_params *p, int64_t nobs, int
         t_last = now;
     };
     h->p = *p;
+    h->objective = p->loss >= EVB_DISTILL ? p->loss : 0;
+    h->p.loss = evb_rules_of(p->loss);
     h->K = p->K; h->C = 2 * p->K + 1; h->B = p->nbins; h->D = p->max_depth; h->nn = (1 << p->max_depth) - 1;
     h->Ce = (p->loss == EVB_MSE && !getenv("EVB_NO_ELISION")) ? p->K + 1 : h->C;
     h->nfeats = nfeats; h->RS = nfeats <= 16 ? 16 : (nfeats + 31) / 32 * 32; h->n = nobs;
@@ -336,7 +338,7 @@ static int32_t create_impl(evb_handle *h, const evb_params *p, int64_t nobs, int
         phase("rows of bins");
     }
     {
-        const size_t ybytes = (size_t)n * (y_dtype == EVB_U32 ? 4 : 4 * (size_t)ycols);
+        const size_t ybytes = (size_t)n * 4 * (y_dtype == EVB_U32 && !h->objective ? 1 : (size_t)ycols);
         EVB_CUDA(evb_dev_alloc(&h->y, ybytes ? ybytes : 1));
         EVB_CHECK(evb_h2d_staged(h->y, y, ybytes, h->st, false));
         float *w_d = nullptr, *p0_d = nullptr, *mu_d = nullptr;
@@ -390,13 +392,14 @@ static int32_t create_common(evb_handle **out, const evb_params *p, int64_t nobs
     if (p->loss < 0 || p->loss > EVB_LOSS_LAST) { evb_set_error("evb_create: unknown loss %d", p->loss); return EVB_ERR_ARG; }
     if (p->K < 1 || p->K > 32) { evb_set_error("evb_create: K=%d outside 1..32", p->K); return EVB_ERR_ARG; }
     const bool mle = p->loss == EVB_GAUSSIAN_MLE || p->loss == EVB_LOGISTIC_MLE;
-    if ((mle && (p->K % 2 != 0 || ycols != p->K / 2)) || (!mle && p->loss != EVB_MLOGLOSS && p->loss != EVB_MULTIQUANTILE && ycols != p->K) ||
+    if (p->loss >= EVB_DISTILL) EVB_CHECK(evb_check_objective(p, nobs, y_dtype, ycols));
+    else if ((mle && (p->K % 2 != 0 || ycols != p->K / 2)) || (!mle && p->loss != EVB_MLOGLOSS && p->loss != EVB_MULTIQUANTILE && ycols != p->K) ||
         (p->loss == EVB_MULTIQUANTILE && (ycols != 1 || p->K > 8)) ||
         (p->loss == EVB_MLOGLOSS && p->K < 2)) {
         evb_set_error("evb_create: K=%d / ycols=%d inconsistent with the loss", p->K, ycols);
         return EVB_ERR_ARG;
     }
-    if ((p->loss == EVB_MLOGLOSS) != (y_dtype == EVB_U32) || (y_dtype != EVB_U32 && y_dtype != EVB_F32)) {
+    if (p->loss < EVB_DISTILL && (p->loss == EVB_MLOGLOSS) != (y_dtype == EVB_U32) || (y_dtype != EVB_U32 && y_dtype != EVB_F32)) {
         evb_set_error("evb_create: y_dtype must be EVB_U32 for mlogloss and EVB_F32 otherwise");
         return EVB_ERR_ARG;
     }
@@ -463,6 +466,7 @@ extern "C" int32_t evb_comm_init(evb_handle *h, const uint8_t id[128], int32_t r
     if (!id || world < 1 || rank < 0 || rank >= world) { evb_set_error("evb_comm_init: bad rank/world"); return EVB_ERR_ARG; }
     if (h->nccl_comm || h->nccl_pending) { evb_set_error("evb_comm_init: communicator already initialised"); return EVB_ERR_ARG; }
     if (world == 1) return EVB_OK;
+    if (h->objective) { evb_set_error("evb_comm_init: distill, policy and preference are for one GPU"); return EVB_ERR_ARG; }
     if (!h->hcomp) EVB_CUDA(dalloc(&h->hcomp, (size_t)h->maxslots * h->nfeats * h->C * h->B));
     drop_graphs(h);
     h->gradq_valid = false; // the level kernels' words: trees grown in one launch have not made them
@@ -504,7 +508,8 @@ static int32_t enqueue_tree(evb_handle *h, int use_mask, uint8_t mask_cond, bool
         EVB_CHECK(evb_launch_quantile_leaves(h, use_mask != EVB_MASK_NONE, mask_cond));
         EVB_CHECK(evb_launch_finalize(h, fuse, 2, pub));
     } else {
-        EVB_CHECK(evb_launch_finalize(h, fuse, 0, pub));
+        EVB_CHECK(evb_launch_finalize(h, fuse && !h->objective, 0, pub));
+        if (fuse && h->objective) EVB_CHECK(evb_launch_grads(h));
     }
     if (h->ev_n > 0) EVB_CHECK(evb_launch_eval(h, nullptr, h->h_tree[slot]));
     return EVB_OK;
@@ -684,7 +689,8 @@ static int32_t eval_attach_impl(evb_handle *h, int64_t nobs, const uint8_t *x_bi
     EVB_CUDA(dalloc(&h->ev_xT, (size_t)nobs * h->RS));
     EVB_CUDA(dalloc(&h->ev_pred, (size_t)nobs * K));
     EVB_CUDA(dalloc(&h->ev_part, (size_t)std::max(h->ev_blocks, h->num_sms) * 2));
-    const size_t ybytes = (size_t)nobs * (h->y_dtype == EVB_U32 ? 4 : 4 * (size_t)h->ycols);
+    if (h->objective) EVB_CUDA(dalloc(&h->ev_loss, (size_t)nobs));
+    const size_t ybytes = (size_t)nobs * 4 * (h->y_dtype == EVB_U32 && !h->objective ? 1 : (size_t)h->ycols);
     EVB_CUDA(evb_dev_alloc(&h->ev_y, ybytes));
     EVB_CHECK(evb_h2d_staged(h->ev_y, y, ybytes, h->st, false));
     if (w) {
@@ -738,12 +744,13 @@ static int32_t eval_attach(evb_handle *h, int64_t nobs, const uint8_t *x_bin, co
     if (h->pending > 0) { evb_set_error("evb_eval_attach: a tree is still in flight"); return EVB_ERR_BUSY; }
     if (h->ev_n > 0) { evb_set_error("evb_eval_attach: evaluation data already attached (evb_eval_detach first)"); return EVB_ERR_ARG; }
     const int loss = h->p.loss;
-    const bool ok = (loss == EVB_MLOGLOSS) ? metric == EVB_METRIC_MLOGLOSS
+    const bool ok = h->objective ? metric == EVB_METRIC_DISTILL + (h->objective - EVB_DISTILL) : (loss == EVB_MLOGLOSS) ? metric == EVB_METRIC_MLOGLOSS
                     : (loss == EVB_GAUSSIAN_MLE || loss == EVB_LOGISTIC_MLE) ? (metric == EVB_METRIC_GAUSSIAN_MLE || metric == EVB_METRIC_LOGISTIC_MLE)
                     : (metric == EVB_METRIC_MSE || metric == EVB_METRIC_MAE || metric == EVB_METRIC_LOGLOSS ||
                        metric == EVB_METRIC_POISSON || metric == EVB_METRIC_GAMMA || metric == EVB_METRIC_TWEEDIE ||
                        metric == EVB_METRIC_QUANTILE || (metric == EVB_METRIC_MULTIQUANTILE && loss == EVB_MULTIQUANTILE));
-    if (!ok) { evb_set_error("evb_eval_attach: metric %d is not defined for loss %d", metric, loss); return EVB_ERR_ARG; }
+    if (!ok) { evb_set_error("evb_eval_attach: metric %d is not defined for loss %d", metric, h->objective ? h->objective : loss); return EVB_ERR_ARG; }
+    if (h->objective == EVB_PREFERENCE && nobs % 2 != 0) { evb_set_error("evb_eval_attach: preferences need an even number of rows"); return EVB_ERR_ARG; }
     drop_graphs(h); // the launch sequence of a tree changes
     int32_t rc = eval_attach_impl(h, nobs, x_bin, mx, y, w, pred0, bias, metric, sums);
     if (rc != EVB_OK) free_eval(h);

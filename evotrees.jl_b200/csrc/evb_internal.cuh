@@ -82,7 +82,8 @@ struct GrowGeom {
 };
 
 struct evb_handle {
-    evb_params p;
+    evb_params p;              // p.loss: whose rules for leaves, gains and records hold (evb_rules_of)
+    int objective;             // 0, or the loss whose gradients evb_softrow.cu makes (EVB_DISTILL and up)
     int K, C, B, D, nn;        // nn = 2^D-1
     int Ce;                    // channels of a record with its weight: C, or K+1 for mse where h = 2w is rebuilt from w
     int nfeats, RS;            // RS: bytes per row of xT (16, or a multiple of 32)
@@ -143,6 +144,7 @@ struct evb_handle {
     uint8_t *ev_xT;    // [ev_n][RS]
     void *ev_y; float *ev_w; float *ev_pred;
     double *ev_part;   // [ev_blocks][2] per-block partial sums
+    float *ev_loss;    // [ev_n] losses of the rows (objective)
     double *d_evsum;   // [2] inside the tree block: sum w*value, sum w
     int ev_metric, ev_blocks;
     double last_eval[2]; // sums of the tree collected last
@@ -238,6 +240,15 @@ int32_t evb_launch_rows_init(evb_handle *h, int use_mask, uint8_t mask_cond);
 int32_t evb_pcg_tables(int dev);
 void evb_pcg_advance(uint64_t gen[6], int64_t n);
 int32_t evb_launch_finalize(evb_handle *h, bool compute_grads, int mode, void *publish_to); // pinned host memory for the finished tree or null; mode: see FinArgs in evb_rows.cu
+int32_t evb_launch_absmax(evb_handle *h); // evb_rows.cu: maxima of the gradients in place
+int32_t evb_launch_loss_sums(evb_handle *h, int64_t n, int w_step); // of ev_loss, into ev_part
+// evb_softrow.cu: gradients of the training rows, or losses of the evaluation rows, of h->objective
+int32_t evb_launch_objective(evb_handle *h, bool eval);
+int32_t evb_check_objective(const evb_params *p, int64_t nobs, int32_t y_dtype, int32_t ycols);
+// The losses that evb_softrow.cu makes the gradients of follow another loss in the rest: classes add up and are linked as for mlogloss; scores add up,
+// with gradient and hessian in the gain, as for poisson, and are not linked, as for mse.
+static inline int evb_rules_of(int loss) { return loss == EVB_PREFERENCE ? EVB_POISSON : loss >= EVB_DISTILL ? EVB_MLOGLOSS : loss; }
+static inline int evb_link_of(int loss) { return loss == EVB_PREFERENCE ? EVB_MSE : loss >= EVB_DISTILL ? EVB_MLOGLOSS : loss; }
 int32_t evb_launch_quantile_leaves(evb_handle *h, bool use_mask, uint8_t mask_cond);
 int32_t evb_launch_nidx_from_partition(evb_handle *h, uint32_t *out_dev);
 int32_t evb_launch_eval(evb_handle *h, const float *fixed_leaf_dev, void *publish_to);

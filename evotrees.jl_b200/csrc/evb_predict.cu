@@ -756,7 +756,7 @@ extern "C" int32_t evb_model_create(evb_model **out, int32_t device, int32_t los
     EVB_CHECK(evb_check_device(device));
     evb_model *m = new (std::nothrow) evb_model();
     if (!m) { evb_set_error("out of host memory"); return EVB_ERR_ARG; }
-    m->device = device; m->loss = loss; m->K = K;
+    m->device = device; m->loss = evb_link_of(loss); m->K = K;
     int32_t rc;
     try { rc = model_fill(m, ntrees, src, nodes, edges, edges_dtype, nedges, nfeats, feattypes, true); }
     catch (const std::bad_alloc &) { rc = no_host_memory(); }
@@ -1083,7 +1083,7 @@ static int32_t predict_once(int32_t device, int32_t loss, int32_t K, int32_t ntr
     EVB_CHECK(evb_check_device(device));
     if (nobs == 0) return EVB_OK;
     evb_model m;
-    m.device = device; m.loss = loss; m.K = K;
+    m.device = device; m.loss = evb_link_of(loss); m.K = K;
     int32_t rc;
     try {
         std::vector<const void *> src((size_t)ntrees * 4);

@@ -70,6 +70,12 @@ __global__ void __launch_bounds__(256) k_grads(int loss, int K, int nq, int unit
     block_absmax(rec, ng, gmax);
 }
 
+// the same of gradients that another kernel has made
+__global__ void __launch_bounds__(256) k_absmax(const float *grad, long long n, int nq, unsigned *gmax, int ng) {
+    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    block_absmax(i < n ? grad + (size_t)i * nq : nullptr, ng, gmax);
+}
+
 // ---------------------------------------------------------------------------------- row sampling
 constexpr int SEL_CHUNK = 2048, SEL_THREADS = 256;
 __global__ void __launch_bounds__(SEL_THREADS) k_sel_count(const uint8_t *mask, uint8_t cond, long long n, int32_t *bcnt) {
@@ -561,7 +567,7 @@ __global__ void __launch_bounds__(256) k_eval_tree(EvalArgs a) {
         const float *leaf = a.fixed_leaf ? a.fixed_leaf : a.t_pred + (size_t)(traverse(packed, a.xT + (size_t)i * a.RS) - 1) * a.K;
         pred_add(a.loss, a.K, p, leaf);
         const float w = a.w ? a.w[i] : 1.0f;
-        sv += (double)metric_row(a.metric, a.K, p, a.y, a.ycols, i, w, a.alpha);
+        if (a.metric >= 0) sv += (double)metric_row(a.metric, a.K, p, a.y, a.ycols, i, w, a.alpha); // else by the kernels of an objective
         sw += (double)w;
     }
     for (int o = 16; o > 0; o >>= 1) { sv += __shfl_down_sync(FULL, sv, o); sw += __shfl_down_sync(FULL, sw, o); }
@@ -589,9 +595,39 @@ __global__ void __launch_bounds__(256) k_eval_sum(const double *part, int nblock
     publish(pub_src, pub_dst, pub_n);
 }
 
+// sums of losses that another kernel has made (w is in them) and of the weights of every w_step-th row; blocks as k_eval_tree
+__global__ void __launch_bounds__(256) k_loss_sums(const float *loss, const float *w, long long n, int w_step, double *part) {
+    __shared__ double s_red[2][8];
+    double sv = 0.0, sw = 0.0;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+        sv += (double)loss[i];
+        sw += w ? (double)w[i * w_step] : 1.0;
+    }
+    sv = warp_sum(sv); sw = warp_sum(sw);
+    if ((threadIdx.x & 31) == 0) { s_red[0][threadIdx.x >> 5] = sv; s_red[1][threadIdx.x >> 5] = sw; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double tv = 0.0, tw = 0.0;
+        for (int q = 0; q < 8; ++q) { tv += s_red[0][q]; tw += s_red[1][q]; }
+        part[2 * blockIdx.x] = tv;
+        part[2 * blockIdx.x + 1] = tw;
+    }
+}
+
 } // namespace
 
 // =====================================================================================================
+int32_t evb_launch_absmax(evb_handle *h) {
+    k_absmax<<<(unsigned)((h->n + 255) / 256), 256, 0, h->st>>>(h->grad, h->n, h->nq, evb_gmax(h, false), h->ng);
+    EVB_CUDA(cudaGetLastError());
+    return EVB_OK;
+}
+int32_t evb_launch_loss_sums(evb_handle *h, int64_t n, int w_step) {
+    k_loss_sums<<<h->ev_blocks, 256, 0, h->st>>>(h->ev_loss, h->ev_w, n, w_step, h->ev_part);
+    EVB_CUDA(cudaGetLastError());
+    return EVB_OK;
+}
+
 int32_t evb_launch_transpose(evb_handle *, const uint8_t *xcol_dev, int64_t ld, int64_t nrows, int j0, int nj, uint8_t *xT,
                              int RS, cudaStream_t st) {
     dim3 grid((unsigned)((nrows + 255) / 256), (unsigned)((nj + 3) / 4));
@@ -617,6 +653,13 @@ int32_t evb_launch_init_state(evb_handle *h, const float *w_dev, const float *pr
 int32_t evb_launch_grads(evb_handle *h) {
     EVB_CUDA(cudaMemsetAsync(evb_gmax(h, false), 0, sizeof(unsigned) * h->ng, h->st));
     evb_tic(h, EVB_T_GRADS);
+    if (h->objective) {
+        const int32_t rc = evb_launch_objective(h, false);
+        if (rc == EVB_OK) EVB_CHECK(evb_launch_absmax(h));
+        evb_toc(h, EVB_T_GRADS);
+        h->tm.launches[EVB_T_GRADS] += 1; // two kernels inside one timed bracket
+        return rc;
+    }
     k_grads<<<(unsigned)((h->n + 255) / 256), 256, 0, h->st>>>(h->p.loss, h->K, h->nq, h->unit_w ? 1 : 0, h->Ce != h->C, h->ycols, h->n, h->pred, h->y, h->grad,
                                                                 evb_gmax(h, false), h->ng, evb_alpha_set(h));
     evb_toc(h, EVB_T_GRADS);
@@ -749,11 +792,17 @@ int32_t evb_launch_eval(evb_handle *h, const float *fixed_leaf_dev, void *publis
     EvalArgs a;
     a.xT = h->ev_xT; a.t_packed = h->t_packed; a.t_pred = h->t_pred; a.fixed_leaf = fixed_leaf_dev; a.pred = h->ev_pred;
     a.y = h->ev_y; a.w = h->ev_w; a.part = h->ev_part; a.n = h->ev_n; a.RS = h->RS; a.K = h->K; a.loss = h->p.loss;
-    a.metric = h->ev_metric; a.nn = h->nn; a.ycols = h->ycols; a.alpha = evb_alpha_set(h);
+    a.metric = h->objective ? -1 : h->ev_metric; a.nn = h->nn; a.ycols = h->ycols; a.alpha = evb_alpha_set(h);
     const size_t smem = (size_t)h->nn * 4;
     a.packed_in_smem = smem <= 40 * 1024 ? 1 : 0;
     evb_tic(h, EVB_T_FINALIZE);
     k_eval_tree<<<h->ev_blocks, 256, (a.packed_in_smem && !fixed_leaf_dev) ? smem : 0, h->st>>>(a);
+    if (h->objective) {
+        const bool pairs = h->objective == EVB_PREFERENCE;
+        EVB_CHECK(evb_launch_objective(h, true));
+        EVB_CHECK(evb_launch_loss_sums(h, pairs ? h->ev_n / 2 : h->ev_n, pairs ? 2 : 1));
+        h->tm.launches[EVB_T_FINALIZE] += 2;
+    }
     k_eval_sum<<<1, 256, 0, h->st>>>(h->ev_part, h->ev_blocks, h->d_evsum, reinterpret_cast<const uint4 *>(h->plan), static_cast<uint4 *>(publish_to),
                                      publish_to ? (int)(h->h_tree_bytes / 16) : 0);
     evb_toc(h, EVB_T_FINALIZE);

@@ -1424,6 +1424,64 @@ bool good_tau(double v) { return v >= 1.0e-6 && v <= 1.0e6; }
 
 } // namespace
 
+// ---------------------------------------------------------------------------------- as losses of a handle
+namespace {
+// Rows 2 p and 2 p + 1 of one output: the scores are log ratios already, less those of the reference
+__global__ void __launch_bounds__(256) k_score_pairs(const float *pred, const float *ref, const float *w, long long w_stride, long long pairs, float beta, float smooth,
+                                                     float *grad, int nq, float *loss) {
+    const long long p = (long long)blockIdx.x * blockDim.x + threadIdx.x, i = 2 * p;
+    if (p >= pairs) return;
+    const float m = beta * ((pred[i] - ref[i]) - (pred[i + 1] - ref[i + 1])), wp = w ? w[i * w_stride] : 1.0f;
+    const RowLoss o = pair_loss(m, wp, smooth);
+    if (loss) loss[p] = o.loss;
+    if (grad) {
+        const float g = beta * o.d, h = wp * beta * beta / ((1.0f + expf(-m)) * (1.0f + expf(m)));
+        grad[i * nq] = g; grad[i * nq + 1] = h;
+        grad[(i + 1) * nq] = -g; grad[(i + 1) * nq + 1] = h;
+    }
+}
+} // namespace
+
+int32_t evb_check_objective(const evb_params *p, int64_t nobs, int32_t y_dtype, int32_t ycols) {
+    const double *q = p->alphas;
+    const bool pref = p->loss == EVB_PREFERENCE, dist = p->loss == EVB_DISTILL;
+    if (pref ? p->K != 1 || y_dtype != EVB_F32 || ycols != 1 || nobs % 2 != 0 : p->K < 2 || y_dtype != EVB_U32 || (dist ? ycols < 2 || ycols % 2 != 0 || ycols > 2 * MAX_TOP : ycols != 4)) {
+        evb_set_error("evb_create: K=%d / ycols=%d / y_dtype=%d / nobs=%lld inconsistent with the loss", p->K, ycols, y_dtype, (long long)nobs);
+        return EVB_ERR_ARG;
+    }
+    const bool ok = pref ? q[0] >= 0.0 && q[0] <= 1.0e6 && q[1] >= 0.0 && q[1] <= 1.0
+                  : dist ? good_tau(q[0]) && (q[1] == 0.0 || (q[1] == 1.0 && q[0] == 1.0))
+                         : good_tau(q[0]) && q[1] >= 0.0 && q[1] <= 1.0 && q[2] >= 0.0 && q[2] <= 3.0e38 && q[3] >= 0.0 && q[3] <= 3.0e38;
+    if (!ok) { evb_set_error("evb_create: parameters of the loss out of range (%g, %g, %g, %g)", q[0], q[1], q[2], q[3]); return EVB_ERR_ARG; }
+    return EVB_OK;
+}
+
+int32_t evb_launch_objective(evb_handle *h, bool eval) {
+    const double *q = h->p.alphas;
+    const int64_t n = eval ? h->ev_n : h->n;
+    const float *pred = eval ? h->ev_pred : h->pred, *w = eval ? h->ev_w : h->unit_w ? nullptr : h->grad + h->nq - 1;
+    const void *y = eval ? h->ev_y : h->y;
+    float *loss = eval ? h->ev_loss : nullptr, *grad = eval ? nullptr : h->grad;
+    const long long ws = eval ? 1 : h->nq;
+    if (h->objective == EVB_PREFERENCE) {
+        k_score_pairs<<<(unsigned)((n / 2 + 255) / 256), 256, 0, h->st>>>(pred, static_cast<const float *>(y), w, ws, n / 2, (float)q[0], (float)q[1], grad, h->nq, loss);
+        EVB_CUDA(cudaGetLastError());
+        return EVB_OK;
+    }
+    SoftArgs a = rows_args(pred, n, h->K, h->K, w, (float)q[0], loss, grad, h->nq, grad ? grad + h->K : nullptr, h->nq);
+    a.w_stride = ws;
+    const uint32_t *words = static_cast<const uint32_t *>(y);
+    if (h->objective == EVB_DISTILL) {
+        a.T = h->ycols / 2; a.ldt = h->ycols; a.tail = q[1] != 0.0;
+        a.ids = words; a.t = words + a.T; a.t_dtype = EVB_F32;
+        return launch_rows<ROW_DISTILL>(a, EVB_F32, h->dev, h->st);
+    }
+    const float *f = reinterpret_cast<const float *>(words);
+    a.code = words; a.p_stride = 4; a.old_lp = f + 1; a.adv = f + 2; a.ref = q[3] > 0.0 ? f + 3 : nullptr;
+    a.lo = (float)q[1]; a.hi = (float)q[2]; a.beta = (float)q[3];
+    return launch_rows<ROW_POLICY>(a, EVB_F32, h->dev, h->st);
+}
+
 extern "C" int32_t evb_distill_grads(int32_t device, void *stream, const void *z, int32_t dtype, int64_t n, int32_t K, int64_t ldz, const uint32_t *ids,
                                      const void *teacher, int32_t teacher_dtype, int32_t T, int32_t tail, const float *w, double tau, float *loss,
                                      void *grad, int64_t ldg, void *hess, int64_t ldh) {

@@ -14,7 +14,7 @@ import numpy as np
 
 from . import _lib
 from .binning import RawMatrix, binarize, get_edges, sample_rows
-from .learners import EvoTypes
+from .learners import OBJECTIVES, EvoTypes
 from .model import EvoTree, Tree
 
 
@@ -111,6 +111,71 @@ def init_target(loss: str, y_train: np.ndarray, offset, alphas=(0.1, 0.5, 0.9)):
     return K, y, ycols, mu.astype(np.float32), levels, offset
 
 
+def pack_objective(params: EvoTypes, y, nobs: int, K: int = 0):
+    """Targets of the losses of `OBJECTIVES` as the library takes them (include/evb.h, evb_create), checked.  Returns K, y, ycols.
+
+    distill     (ids [nobs, slots], values [nobs, slots]): class codes 1..K, 0 = empty; the teacher's logits (`tail`: log-probabilities)
+    policy      (action [nobs], old_logp [nobs], advantage [nobs][, ref_logp [nobs]]); action 0: the row does not count
+    preference  scores of the reference [nobs], or None for zeros; rows 0, 2, .. are preferred to rows 1, 3, .."""
+    if params.loss == "preference":
+        y = np.zeros(nobs, np.float32) if y is None else np.ascontiguousarray(y, np.float32)
+        if y.shape != (nobs,) or nobs % 2:
+            raise ValueError("preference takes an even number of rows (preferred, other, ..) and one reference score a row")
+        if not np.isfinite(y).all():
+            raise ValueError("preference takes finite reference scores")
+        return 1, y, 1
+    want = (2,) if params.loss == "distill" else (3, 4)
+    if not isinstance(y, (tuple, list)) or len(y) not in want:
+        raise ValueError("distill takes (ids, values), policy (action, old_logp, advantage[, ref_logp])")
+    codes = np.asarray(y[0])
+    if not np.issubdtype(codes.dtype, np.integer) or codes.shape[:1] != (nobs,) or codes.ndim != (2 if params.loss == "distill" else 1):
+        raise ValueError("class codes must be integers, one row of them per observation")
+    top = int(codes.max(initial=0))
+    K = K or params.nclasses or top
+    if codes.min(initial=0) < 0 or top > K:
+        raise ValueError(f"class codes must lie within 0..{K}")
+    if not 2 <= K <= 32:
+        raise ValueError(f"{params.loss} takes 2 to 32 classes, got {K}")
+    values = [np.asarray(v, np.float32) for v in y[1:]]
+    if any(v.shape != codes.shape for v in values):
+        raise ValueError("codes and values must have the same shape")
+    if any(np.isnan(v).any() for v in values):
+        raise ValueError("values must not be NaN")
+    if params.loss == "policy" and len(values) == 2:
+        if params.beta > 0.0:
+            raise ValueError("beta > 0 needs ref_logp as a fourth part of the target")
+        values.append(np.zeros(nobs, np.float32))
+    parts = [codes.reshape(nobs, -1).astype(np.uint32)] + [np.ascontiguousarray(v.reshape(nobs, -1)).view(np.uint32) for v in values]
+    if params.loss == "distill" and not 1 <= parts[0].shape[1] <= 1024:
+        raise ValueError("distill takes 1 to 1024 slots a row")
+    out = np.ascontiguousarray(np.concatenate(parts, axis=1))
+    return K, out, out.shape[1]
+
+
+def init_objective(params: EvoTypes, y_train, offset, nobs: int):
+    """`init_target` for the losses of `OBJECTIVES`: the bias of distill is the logarithm of the teacher's mean probabilities, that of the others
+    zero (all classes alike)."""
+    K, y, ycols = pack_objective(params, y_train, nobs)
+    if params.loss == "preference":
+        return K, y, ycols, np.zeros(1, np.float32), None, offset
+    mu = np.zeros(K, np.float64)
+    if params.loss == "distill":
+        T = ycols // 2
+        ids, t = y[:, :T].astype(np.int64), y[:, T:].view(np.float32).astype(np.float64)
+        t = np.where(ids > 0, t, -np.inf)
+        if params.tail:
+            q = np.exp(t)
+        else:
+            m = t.max(axis=1, keepdims=True)
+            q = np.exp((t - np.where(np.isfinite(m), m, 0.0)) / params.tau)
+            q /= np.maximum(q.sum(axis=1, keepdims=True), 1e-300)
+        p = np.bincount(ids.ravel(), weights=q.ravel(), minlength=K + 1)[1:]
+        p += max(0.0, nobs - p.sum()) / K if params.tail else 0.0
+        mu = np.log(np.maximum(p / max(p.sum(), 1e-300), 1e-7))
+        mu = np.maximum(mu - mu.max(), -15.0)
+    return K, y, ycols, mu.astype(np.float32), np.arange(1, K + 1), None if offset is None else np.log(offset)
+
+
 class Cache:
     """Training cache: owns the device handle (counterpart of `CacheBaseGPU`,
     ext/EvoTreesKernelAbstractionsExt/structs.jl).  It survives `fit` so that boosting can be resumed
@@ -125,6 +190,7 @@ class Cache:
         self.use_mask = False
         self.K = 1
         self.nn = 0
+        self.ycols = 1
         self.feature_names = None
         self.edges = None           # edges the handle keeps (made from a RawMatrix), else None
 
@@ -192,10 +258,15 @@ def make_rngs(seed: int, rank: int = 0):
     return np.random.default_rng([seed, rank]), np.random.default_rng([seed, 0x6A73])
 
 
+def objective_parameters(params: EvoTypes):
+    return {"distill": (params.tau, float(params.tail)), "policy": (params.tau, *params.clip, params.beta),
+            "preference": (params.beta, params.smooth)}.get(params.loss)
+
+
 def make_params(params: EvoTypes, K: int, device: int, flags: int = 0) -> _lib.EvbParams:
     return _lib.EvbParams(_lib.LOSS_CODES[params.loss], K, params.nbins, params.max_depth, params.bagging_size,
                           1 if params.tree_type == "oblivious" else 0, params.eta, params.lambda_, params.L2, params.gamma, params.min_weight, device, flags, params.alpha,
-                          (C.c_double * 8)(*(list(params.alphas) + [0.0] * 8)[:8]))
+                          (C.c_double * 8)(*(list(objective_parameters(params) or params.alphas) + [0.0] * 8)[:8]))
 
 
 def init_core_binned(params: EvoTypes, x_bin: np.ndarray, y, ycols: int, K: int, mu: np.ndarray, w=None, pred0=None,
@@ -213,6 +284,7 @@ def init_core_binned(params: EvoTypes, x_bin: np.ndarray, y, ycols: int, K: int,
         nobs, nfeats = x_raw.shape
     cache = Cache()
     cache.nobs, cache.nfeats, cache.K, cache.nn = nobs, nfeats, K, 2 ** params.max_depth - 1
+    cache.ycols = ycols
     cache.njs = math.ceil(params.colsample * nfeats)            # src/init.jl:181
     cache.mask_cond = int(np.uint8(round(255 * params.rowsample)))  # src/subsample.jl:9
     cache.use_mask = params.rowsample < 1.0
@@ -224,9 +296,11 @@ def init_core_binned(params: EvoTypes, x_bin: np.ndarray, y, ycols: int, K: int,
     w32 = None if w is None else np.ascontiguousarray(w, np.float32)
     if w32 is not None and (w32.size != nobs or w32.min() <= 0):
         raise ValueError("weights must be positive and of length nobs")   # src/init.jl:165
+    if w32 is not None and params.loss == "preference" and not np.array_equal(w32[0::2], w32[1::2]):
+        raise ValueError("the two rows of a pair must have the same weight")
     p0 = None if pred0 is None else np.ascontiguousarray(pred0, np.float32)
     cp = make_params(params, K, device, flags)
-    ydt = _lib.EVB_U32 if params.loss == "mlogloss" else _lib.EVB_F32
+    ydt = _lib.EVB_U32 if params.loss in ("mlogloss", "distill", "policy") else _lib.EVB_F32
     mu32 = np.ascontiguousarray(mu, np.float32)
     if x_raw is None and matrix is None:
         _lib.check(_lib.lib().evb_create(C.byref(cache.handle), C.byref(cp), C.c_int64(nobs), C.c_int32(nfeats), _lib.ptr(x_bin),
@@ -262,6 +336,8 @@ def init_core(params: EvoTypes, x_train: np.ndarray, y_train, w_train=None, offs
     if x_train.dtype not in (np.float32, np.float64):
         x_train = x_train.astype(np.float64)
     nobs, nfeats = x_train.shape
+    if comm is not None and params.loss in OBJECTIVES:
+        raise ValueError(f"`{params.loss}` is for one GPU")
     rng = np.random.default_rng(params.seed)
     host = {}
 
@@ -269,7 +345,8 @@ def init_core(params: EvoTypes, x_train: np.ndarray, y_train, w_train=None, offs
         try:
             host["rows"] = sample_rows(nobs, params.nbins, rng)
             offset = None if offset_train is None else np.array(offset_train, np.float32, copy=True).reshape(nobs, -1)
-            host["target"] = init_target(params.loss, y_train, offset, params.alphas)
+            host["target"] = init_objective(params, y_train, offset, nobs) if params.loss in OBJECTIVES else \
+                init_target(params.loss, y_train, offset, params.alphas)
         except Exception as e:
             host["error"] = e
 
@@ -436,7 +513,8 @@ def grow_evotree(m: EvoTree, cache: Cache, params: EvoTypes) -> None:
 
 IS_MAXIMISE = {"mse": False, "rmse": False, "mae": False, "logloss": False, "mlogloss": False, "poisson": False,
                "gamma": False, "tweedie": False, "quantile": False, "multiquantile": False, "gaussian_mle": True,
-               "logistic_mle": True}   # src/metrics.jl:194-205
+               "logistic_mle": True,   # src/metrics.jl:194-205
+               "distill": False, "policy": False, "preference": False}
 
 
 def init_logger(metric: str, maximise: bool, early_stopping_rounds: int, early_stopping_tolerance: float = 0.0) -> dict:
@@ -513,17 +591,24 @@ class CallBack:
         loss, K = params.loss, m.K
         if loss == "mlogloss":
             y = eval_levelcode(y_eval, m.info["target_levels"])
+        elif loss in OBJECTIVES:
+            y = pack_objective(params, y_eval, nobs, K)
+            if y[2] != cache.ycols:
+                raise ValueError("y_eval must have as many slots as y_train")
+            y = y[1]
         else:
             y = np.ascontiguousarray(y_eval, np.float32)
         if y.shape[0] != nobs:
             raise ValueError("y_eval must have one entry per row of x_eval")
         w = None if w_eval is None else np.ascontiguousarray(w_eval, np.float32)
+        if w is not None and loss == "preference" and not np.array_equal(w[0::2], w[1::2]):
+            raise ValueError("the two rows of a pair must have the same weight")
         pred0 = None
         if offset_eval is not None:                                  # src/callback.jl:110-118
             off = np.array(offset_eval, np.float32, copy=True).reshape(nobs, -1)
             if loss == "logloss":
                 off = _logit(off)
-            elif loss in ("mlogloss", "poisson", "gamma", "tweedie"):
+            elif loss in ("mlogloss", "poisson", "gamma", "tweedie", "distill", "policy"):
                 off = np.log(off)
             elif loss in ("gaussian_mle", "logistic_mle"):
                 off[:, 1::2] = [[_invsoftplus(float(v)) for v in row] for row in off[:, 1::2]]
@@ -571,17 +656,20 @@ class CallBack:
         _lib.check(_lib.lib().evb_eval_detach(self.cache.handle))
 
 
-def fit(params: EvoTypes, *, x_train, y_train, w_train=None, offset_train=None, x_eval=None, y_eval=None, w_eval=None,
+def fit(params: EvoTypes, *, x_train, y_train=None, w_train=None, offset_train=None, x_eval=None, y_eval=None, w_eval=None,
         offset_eval=None, feature_names=None, device: int = 0, return_cache: bool = False, comm=None, **_ignored):
     """`fit(params; x_train, y_train, w_train, offset_train, x_eval, y_eval, w_eval, offset_eval, feature_names)`
     (src/fit.jl:388-437).  With evaluation data the metric of every round is logged in `m.info["logger"]` and
-    boosting stops once `early_stopping_rounds` rounds passed without improvement."""
+    boosting stops once `early_stopping_rounds` rounds passed without improvement.  Targets of the losses distill, policy and
+    preference: `pack_objective`."""
+    if y_train is None and params.loss != "preference":
+        raise ValueError("`y_train` is missing")
     m, cache = init_core(params, x_train, y_train, w_train, offset_train, feature_names, device, comm=comm)
-    if (x_eval is None) != (y_eval is None):
+    if (x_eval is None) != (y_eval is None) and not (params.loss == "preference" and x_eval is not None):
         import warnings
         warnings.warn("To track eval metric in logger, both `x_eval` and `y_eval` must be provided.")
     logger = cb = None
-    if x_eval is not None and y_eval is not None:
+    if x_eval is not None and (y_eval is not None or params.loss == "preference"):
         cb = CallBack(params, m, cache, x_eval, y_eval, w_eval, offset_eval, device, comm)
         logger = init_logger(params.metric, IS_MAXIMISE[params.metric], params.early_stopping_rounds,
                              params.early_stopping_tolerance)

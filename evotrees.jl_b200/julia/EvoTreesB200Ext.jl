@@ -26,7 +26,8 @@ struct EvbParams
 end
 
 const LOSS_CODE = Dict(:mse => 0, :logloss => 1, :mlogloss => 2, :gaussian_mle => 3, :poisson => 4, :gamma => 5, :tweedie => 6, :logistic_mle => 7,
-    :mae => 8, :cred_var => 9, :cred_std => 10, :quantile => 11, :multiquantile => 12)
+    :mae => 8, :cred_var => 9, :cred_std => 10, :quantile => 11, :multiquantile => 12, :distill => 13, :policy => 14, :preference => 15)
+# (the last three have no learner in the reference: they are reached from Python)
 # loss type of a fitted model (the `L` of `EvoTree{L,K}`) -> code: the inverse of the reference's own table (src/loss.jl:20-34)
 const LOSS_TYPE_CODE = Dict(T => LOSS_CODE[s] for (s, T) in _loss2type_dict)
 

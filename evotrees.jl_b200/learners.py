@@ -8,7 +8,9 @@ from __future__ import annotations
 
 from dataclasses import dataclass, field
 
-_REG_LOSSES = ("mse", "logloss", "poisson", "gamma", "tweedie", "mae", "cred_var", "cred_std", "quantile", "multiquantile")
+_REG_LOSSES = ("mse", "logloss", "poisson", "gamma", "tweedie", "mae", "cred_var", "cred_std", "quantile", "multiquantile", "preference")
+# losses whose targets are more than one value a row (no counterpart in the reference); each is its own and only metric
+OBJECTIVES = ("distill", "policy", "preference")
 _MLE_LOSSES = ("gaussian_mle", "logistic_mle")
 
 
@@ -40,6 +42,12 @@ class EvoTypes:
     alpha: float = 0.5          # quantile loss / metric
     alphas: tuple = (0.1, 0.5, 0.9)   # multiquantile loss / metric (src/learners.jl:45)
     metric: str | None = None
+    nclasses: int = 0           # distill, policy: classes (0: the largest code of the target)
+    tau: float = 1.0            # distill, policy: temperature
+    tail: bool = False          # distill: slots hold log-probabilities, all other classes are one more
+    clip: tuple = (0.2, 0.2)    # policy: how far the ratio counts, below and above 1
+    beta: float = 0.1           # policy: weight of the KL term; preference: what a difference of scores counts
+    smooth: float = 0.0         # preference: share of pairs taken to be the wrong way round
 
     _losses = ()
     _metrics = ()
@@ -63,6 +71,8 @@ class EvoTypes:
             self.metric = "logistic_mle"
         if self.metric not in self._metrics:
             raise ValueError(f"Invalid metric. Must be one of: {list(self._metrics)}")
+        if (self.loss in OBJECTIVES or self.metric in OBJECTIVES) and self.metric != self.loss:
+            raise ValueError(f"Invalid metric `{self.metric}` for loss `{self.loss}`")
         self.check_args()
 
     def check_args(self):
@@ -82,6 +92,16 @@ class EvoTypes:
             self.alphas = tuple(float(a) for a in self.alphas)
             if not 1 <= len(self.alphas) <= 8 or any(not 0.0 < a < 1.0 for a in self.alphas):
                 raise ValueError("`alphas` must hold 1 to 8 values strictly between 0 and 1")
+        if self.loss in OBJECTIVES:
+            _check("nclasses", self.nclasses, 0, 32)
+            _check("tau", self.tau, 1e-6, 1e6)
+            _check("beta", self.beta, 0.0, 1e6)
+            _check("smooth", self.smooth, 0.0, 1.0)
+            self.clip = tuple(float(c) for c in self.clip)
+            if len(self.clip) != 2 or not 0.0 <= self.clip[0] <= 1.0 or not 0.0 <= self.clip[1] <= 1e6:
+                raise ValueError("`clip` must hold two values, the first within [0, 1], the second within [0, 1e6]")
+            if self.tail and self.tau != 1.0:
+                raise ValueError("`tail` needs `tau` to be 1")
         self.tree_type = str(self.tree_type).lstrip(":")
         if self.tree_type not in ("binary", "oblivious"):   # src/learners.jl: tree_type ∈ (:binary, :oblivious)
             raise ValueError("Invalid input for `tree_type` parameter: must be `binary` or `oblivious`")
@@ -92,14 +112,15 @@ class EvoTypes:
 @dataclass
 class EvoTreeRegressor(EvoTypes):
     _losses = _REG_LOSSES
-    _metrics = ("mse", "rmse", "mae", "logloss", "poisson", "gamma", "tweedie", "quantile", "multiquantile")
+    _metrics = ("mse", "rmse", "mae", "logloss", "poisson", "gamma", "tweedie", "quantile", "multiquantile",
+                "preference")
 
 
 @dataclass
 class EvoTreeClassifier(EvoTypes):
     loss: str = "mlogloss"
-    _losses = ("mlogloss",)
-    _metrics = ("mlogloss",)
+    _losses = ("mlogloss", "distill", "policy")
+    _metrics = ("mlogloss", "distill", "policy")
 
 
 @dataclass

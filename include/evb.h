@@ -53,8 +53,12 @@ enum evb_status {
 enum evb_loss { EVB_MSE = 0, EVB_LOGLOSS = 1, EVB_MLOGLOSS = 2, EVB_GAUSSIAN_MLE = 3,
                 EVB_POISSON = 4, EVB_GAMMA = 5, EVB_TWEEDIE = 6, EVB_LOGISTIC_MLE = 7,
                 EVB_MAE = 8, EVB_CRED_VAR = 9, EVB_CRED_STD = 10, EVB_QUANTILE = 11,
-                EVB_MULTIQUANTILE = 12 /* one target, K = number of quantiles evb_params.alphas[0..K-1], K <= 8 (src/loss.jl:160-172) */ };
-#define EVB_LOSS_LAST EVB_MULTIQUANTILE
+                EVB_MULTIQUANTILE = 12 /* one target, K = number of quantiles evb_params.alphas[0..K-1], K <= 8 (src/loss.jl:160-172) */,
+                /* the losses of evb_*_grads below (no counterpart in the reference); leaves, clamps and links of the first two are those of mlogloss:
+                 * distillation from a teacher's top logits (evb_params.alphas: tau, tail), clipped policy loss (tau, clip_low, clip_high,
+                 * beta) and, for one output, preferences between neighbouring rows (beta, smooth) */
+                EVB_DISTILL = 13, EVB_POLICY = 14, EVB_PREFERENCE = 15 };
+#define EVB_LOSS_LAST EVB_PREFERENCE
 enum evb_dtype { EVB_F32 = 0, EVB_U32 = 1, EVB_F64 = 2, EVB_BF16 = 3, EVB_F16 = 4 /* the last two: predictions of evb_*_grads only */ };
 
 /* flags of evb_params.flags */
@@ -76,7 +80,7 @@ typedef struct {
     int32_t device;        /* CUDA device ordinal of this shard */
     uint32_t flags;
     double alpha;          /* quantile loss / metric: the target quantile in (0, 1) (src/learners.jl:44); else unused */
-    double alphas[8];      /* multiquantile loss / metric: the K target quantiles (src/learners.jl:45); else unused */
+    double alphas[8];      /* multiquantile loss / metric: the K target quantiles (src/learners.jl:45); parameters of distill, policy, preference; else unused */
 } evb_params;
 
 /* Accumulated device time per kernel class since the last evb_reset_timings (EVB_FLAG_TIMING).  EVB_T_PLAN and EVB_T_D2H stay zero: the
@@ -104,7 +108,10 @@ EVB_API int32_t evb_version(void);
  * uploads the binned matrix, targets, weights and initial predictions of this shard and allocates all
  * training state.
  *   x_bin      host, uint8 [nobs x nfeats] column-major, values 1..nbins (binarize, src/fit-utils.jl:66-72)
- *   y          host; EVB_F32 [ycols x nobs] (ycols = 1 for a vector target) or EVB_U32 class codes 1..K
+ *   y          host; EVB_F32 [ycols x nobs] (ycols = 1 for a vector target) or EVB_U32 class codes 1..K.
+ *              distill: EVB_U32 [2 T x nobs], the class codes of a row's T slots, then the bits of their float values; policy: EVB_U32 [4 x nobs],
+ *              action, then the bits of old_logp, adv, ref_logp (read when beta > 0); preference: EVB_F32 [nobs] scores of the reference, rows
+ *              2 i and 2 i + 1 (from 0) being the preferred and the other of pair i: nobs is even, the weight of a pair that of its first row
  *   w          host float [nobs], > 0, or NULL for ones       (src/init.jl:173-174)
  *   pred0      host float [K x nobs] initial predictions (mu + offset), or NULL with mu != NULL
  *   mu         host float [K] used when pred0 == NULL         (src/init.jl:168-170)
@@ -243,7 +250,8 @@ EVB_API int32_t evb_grow_tree_end(evb_handle *h, int64_t *feat, uint8_t *cond_bi
 enum evb_metric { EVB_METRIC_MSE = 0, EVB_METRIC_MAE = 1, EVB_METRIC_LOGLOSS = 2, EVB_METRIC_MLOGLOSS = 3, EVB_METRIC_GAUSSIAN_MLE = 4,
                   EVB_METRIC_POISSON = 5, EVB_METRIC_GAMMA = 6, EVB_METRIC_TWEEDIE = 7, EVB_METRIC_LOGISTIC_MLE = 8,
                   EVB_METRIC_QUANTILE = 9 /* pinball loss at evb_params.alpha (`wmae`, src/metrics.jl:4-6) */,
-                  EVB_METRIC_MULTIQUANTILE = 10 /* mean pinball loss over evb_params.alphas (src/metrics.jl:120-141) */ };
+                  EVB_METRIC_MULTIQUANTILE = 10 /* mean pinball loss over evb_params.alphas (src/metrics.jl:120-141) */,
+                  EVB_METRIC_DISTILL = 11, EVB_METRIC_POLICY = 12, EVB_METRIC_PREFERENCE = 13 /* their losses, for them alone; the last per pair */ };
 EVB_API int32_t evb_eval_attach(evb_handle *h, int64_t nobs, const uint8_t *x_bin, const void *y, const float *w, const float *pred0,
                                 const float *bias, int32_t metric, double sums[2]);
 EVB_API int32_t evb_eval_sums(evb_handle *h, double sums[2]);
