@@ -71,7 +71,7 @@ def lib() -> C.CDLL:
                                            C.c_void_p, C.c_void_p]
         i4, i8, f8, ptr_ = C.c_int32, C.c_int64, C.c_double, C.c_void_p
         rows = [i4, ptr_, ptr_, i4, i8, i4, i8]
-        _lib.evb_distill_grads.argtypes = rows + [ptr_, ptr_, i4, i4, i4, ptr_, f8, ptr_, ptr_, i8, ptr_, i8]
+        _lib.evb_distill_grads.argtypes = rows + [ptr_, ptr_, i4, i4, i4, ptr_, f8, ptr_, ptr_, i8, ptr_, i8, ptr_]
         _lib.evb_policy_grads.argtypes = rows + [ptr_, ptr_, ptr_, ptr_, ptr_, f8, f8, f8, f8, ptr_, ptr_, ptr_, i8, ptr_, i8]
         _lib.evb_preference_grads.argtypes = rows + [ptr_, ptr_, i4, ptr_, ptr_, f8, f8, i4, ptr_, ptr_, ptr_, ptr_, i8, ptr_]
     return _lib

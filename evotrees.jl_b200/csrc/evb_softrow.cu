@@ -18,6 +18,7 @@ constexpr int MAX_CLASSES = 1 << 20;
 
 enum { ROW_DISTILL = 0, ROW_POLICY = 1, ROW_LOGP = 2, ROW_COEF = 3 };
 
+struct TaughtRow;
 struct SoftArgs {
     const void *z;
     long long n, ldz;
@@ -33,6 +34,7 @@ struct SoftArgs {
     const void *t;
     int T, t_dtype, tail;
     long long ldt;
+    const TaughtRow *taught; // per row, or null
     // policy, preference: the class taken; p_stride elements from row to row
     const uint32_t *code;
     const float *old_lp, *adv, *ref;
@@ -377,12 +379,12 @@ __device__ __forceinline__ float take_far(uint4 (&r)[V], const RowAt<ZT> &at, fl
 struct Slots {
     int *id;            // class, 0-based, -1: none
     float *t, *z;       // what the teacher has, the row's prediction
-    float *q, *lp;      // probability, log p: written by slots_row
-    static constexpr int BYTES = 20;
+    float *q;           // the teacher's probability: written by teach_row
+    static constexpr int BYTES = 16;
     __device__ __forceinline__ Slots(void *p, int T) {
         id = static_cast<int *>(p);
         t = reinterpret_cast<float *>(id + T);
-        z = t + T; q = z + T; lp = q + T;
+        z = t + T; q = z + T;
     }
 };
 constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896341f;
@@ -394,53 +396,66 @@ struct RowOut {
     float hw;           // hessian hw p (1 - p)
     float lp;           // log p of the class taken
     float loss;
+    float all_M, all_ls; // distillation: log2 of the sum over all classes, in two parts
 };
 __device__ __forceinline__ bool first_slot(const Slots &s, int j) {
     for (int i = 0; i < j; ++i) if (s.id[i] == s.id[j]) return false;
     return true;
 }
-// r: what the scan found.  `width` lanes share the slots
-__device__ __forceinline__ RowOut slots_row(const SoftArgs &a, const Slots &s, Soft r, float shift, bool dup, float w, int lane, int width) {
+// What a row's slots say by themselves, before its maximum and sum are known: the sum Q of the teacher's probabilities (1 without a tail), sum q log q,
+// the largest named prediction zn, sum q c (z - zn), and (tail) sum of 2^(c (z - zn)) over the classes named, each of them once
+struct Teach { float Q, H, zn, qz, s; };
+struct alignas(16) TaughtRow { Teach teach; int flags; float tmax, r; }; // slots' flags; their largest logit, 1 / sum
+// `width` lanes share the slots; all of them get the same.  Slots without a class have id -1
+__device__ __forceinline__ Teach teach_row(const SoftArgs &a, const Slots &s, bool dup, int lane, int width) {
     const float c = a.c;
-    float tmax = -INFINITY, zmax = r.m;
-    for (int j = lane; j < a.T; j += width) if (s.id[j] >= 0) { tmax = fmaxf(tmax, s.t[j]); zmax = fmaxf(zmax, s.z[j] - shift); }
+    Teach o = {0.0f, 0.0f, -INFINITY, 0.0f, 0.0f};
+    float tmax = -INFINITY;
+    for (int j = lane; j < a.T; j += width) if (s.id[j] >= 0) { tmax = fmaxf(tmax, s.t[j]); o.zn = fmaxf(o.zn, s.z[j]); }
     if (!a.tail) tmax = lanes_max(tmax, width);
-    zmax = lanes_max(zmax, width);
-    const float base = base_of(zmax, c);
-    float Q = 0.0f, named = 0.0f;
+    o.zn = lanes_max(o.zn, width);
+    const float zn = o.zn == -INFINITY ? 0.0f : o.zn;
     for (int j = lane; j < a.T; j += width) {
         if (s.id[j] < 0) continue;
-        const float e = a.tail ? ex2(s.t[j] * LOG2E) : ex2((s.t[j] - tmax) * c);
+        const float lt = a.tail ? s.t[j] : (s.t[j] - tmax) * a.inv_tau, e = ex2(lt * LOG2E), d = (s.z[j] - zn) * c;
         s.q[j] = e;
-        Q += e;
-        if (a.tail && (!dup || first_slot(s, j))) named += ex2(fmaf(s.z[j] - shift, c, -base));
+        o.Q += e;
+        if (e != 0.0f) { o.H += e * lt; o.qz += e * d; }
+        if (a.tail && (!dup || first_slot(s, j))) o.s += ex2(d);
     }
-    Q = lanes_sum(Q, width);
-    Soft all = r;
-    if (a.tail) all = {zmax, lanes_sum(named, width) + r.s * ex2(rise(r.m, c, base))};
-    const float M = base_of(all.m, c), ls = log2f(all.s), lq = logf(Q), rQ = a.tail ? 1.0f : 1.0f / Q;
-    float loss = 0.0f;
-    for (int j = lane; j < a.T; j += width) {
-        if (s.id[j] < 0) continue;
-        const float lt = a.tail ? s.t[j] : (s.t[j] - tmax) * a.inv_tau - lq, q = s.q[j] * rQ, lp = LN2 * (fmaf(s.z[j] - shift, c, -M) - ls);
-        s.q[j] = q;
-        s.lp[j] = lp;
-        if (q != 0.0f) loss += q * (lt - lp);
-    }
-    loss = lanes_sum(loss, width);
+    o.Q = lanes_sum(o.Q, width); o.H = lanes_sum(o.H, width); o.qz = lanes_sum(o.qz, width);
+    if (a.tail) { o.s = lanes_sum(o.s, width); return o; }
+    const float r = 1.0f / o.Q;
+    for (int j = lane; j < a.T; j += width) if (s.id[j] >= 0) s.q[j] *= r;
+    o.H = o.H * r - logf(o.Q);
+    o.qz *= r;
+    o.Q = 1.0f;
+    return o;
+}
+// r: maximum and sum of the row, less `shift`; with a tail of the classes that have no slot
+__device__ __forceinline__ RowOut finish_row(const SoftArgs &a, const Teach &e, Soft r, float shift, float w) {
+    const float c = a.c, zn = e.zn - shift;
+    const Soft all = a.tail ? join(Soft{zn, e.s}, r, c) : r;
+    const float M = base_of(all.m, c), ls = log2f(all.s);
     // the rest, when there is any: no class is left where every one is named or ruled out
-    const float qt = a.tail && r.m != -INFINITY ? fmaxf(0.0f, 1.0f - Q) : 0.0f;
-    if (qt > 0.0f) loss += qt * (logf(qt) - LN2 * (rise(r.m, c, M) + log2f(r.s) - ls));
+    const float qt = a.tail && r.m != -INFINITY ? fmaxf(0.0f, 1.0f - e.Q) : 0.0f;
     RowOut o;
+    o.loss = e.H - LN2 * (e.qz + (zn == -INFINITY ? e.qz == 0.0f ? 0.0f : zn : (fmaf(zn, c, -M) - ls) * e.Q));
+    if (zn == -INFINITY && e.Q > 0.0f) o.loss = all.m == -INFINITY ? NAN : INFINITY; // nothing that the teacher names is possible
+    if (qt > 0.0f) o.loss += qt * (logf(qt) - LN2 * (rise(r.m, c, M) + log2f(r.s) - ls));
     o.M = base_of(r.m, c);
     o.shift = shift;
-    o.mass = a.tail ? Q + qt : 1.0f;
+    o.mass = e.Q + qt;
+    o.all_M = M;
+    o.all_ls = ls;
     o.B = r.m == -INFINITY ? 0.0f * ls : ex2(rise(r.m, c, M)) / all.s;
     o.A = w * a.tau * (o.mass * o.B - (qt > 0.0f ? qt / r.s : 0.0f));
     o.hw = w;
-    o.loss = w * a.tau * a.tau * loss;
+    o.special = o.lp = 0.0f;
+    o.loss *= w * a.tau * a.tau;
     return o;
 }
+__device__ __forceinline__ float slot_p(const SoftArgs &a, const RowOut &o, float z) { return ex2(fmaf(z - o.shift, a.c, -o.all_M) - o.all_ls); }
 __device__ __forceinline__ float less_p(float lp) { return lp < -0.5f ? 1.0f - ex2(lp * LOG2E) : -expm1f(lp); } // 1 - p, also where p is close to 1
 // what belongs to the class taken, read ahead of its use
 struct Taken { float z, old_lp, adv, ref; };
@@ -534,7 +549,7 @@ __device__ __forceinline__ void put_slot(const SoftArgs &a, const RowAt<ZT> &at,
         q = 0.0f;
         for (int i = j; i < a.T; ++i) if (s.id[i] == s.id[j]) q += s.q[i];
     }
-    const float p = ex2(s.lp[j] * LOG2E);
+    const float p = slot_p(a, o, s.z[j]);
     if (at.g) at.g[s.id[j]] = from_f<ZT>(w * a.tau * (o.mass * p - q));
     if (at.h) at.h[s.id[j]] = from_f<ZT>(o.hw * p * (1.0f - p));
 }
@@ -617,7 +632,11 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
             if (far) { shift = all.m; mine_r = {0.0f, take_far<ZT, V>(r, at, shift, a.c, out, lane, G)}; }
             all = lanes_join(mine_r, a.c, G);
         }
-        if (KIND == ROW_DISTILL) { if (!whole) for (int j = lane; j < a.T; j += G) s.id[j] = -1; __syncwarp(); o = slots_row(a, s, all, shift, flags & SLOT_TWICE, w, lane, G); }
+        if (KIND == ROW_DISTILL) {
+            if (!whole) for (int j = lane; j < a.T; j += G) s.id[j] = -1;
+            __syncwarp();
+            o = finish_row(a, teach_row(a, s, flags & SLOT_TWICE, lane, G), all, shift, w);
+        }
         else if (whole) o = class_row<KIND>(a, all, shift, taken, w);
     }
     if (whole) {
@@ -671,7 +690,7 @@ __device__ __forceinline__ void tile_write(T *dst, long long ld, int rows, int W
 }
 template <typename ZT, int KIND>
 __global__ void __launch_bounds__(TILE) k_row_tile(SoftArgs a, TileGeom ge) {
-    extern __shared__ __align__(16) float s_tile[]; // predictions, then gradients [TILE][Kp]; hessians; slots: five words [TILE][Tp] each
+    extern __shared__ __align__(16) float s_tile[]; // predictions, then gradients [TILE][Kp]; hessians; slots: four words [TILE][Tp] each
     constexpr bool DIST = KIND == ROW_DISTILL;
     const long long row0 = (long long)blockIdx.x * TILE, row = row0 + threadIdx.x;
     const int K = a.K, Kp = ge.Kp, rows = (int)min((long long)TILE, a.n - row0);
@@ -712,7 +731,7 @@ __global__ void __launch_bounds__(TILE) k_row_tile(SoftArgs a, TileGeom ge) {
         if (DIST) {
             s.id = reinterpret_cast<int *>(s_s) + threadIdx.x * ge.Tp;
             s.t = s_s + (TILE + threadIdx.x) * ge.Tp;
-            s.z = s.t + TILE * ge.Tp; s.q = s.z + TILE * ge.Tp; s.lp = s.q + TILE * ge.Tp;
+            s.z = s.t + TILE * ge.Tp; s.q = s.z + TILE * ge.Tp;
             for (int j = 0; j < T && live; ++j) {
                 const uint32_t k = (uint32_t)s.id[j];
                 const bool use = k != 0u && s.t[j] != -INFINITY, ok = use && k <= (uint32_t)K;
@@ -747,7 +766,7 @@ __global__ void __launch_bounds__(TILE) k_row_tile(SoftArgs a, TileGeom ge) {
                 z[k] = e;
             }
             const float zero = m == -INFINITY ? m : 0.0f; // the maximum, less itself
-            if (DIST) { o = slots_row(a, s, Soft{zero, sum}, base, flags & SLOT_TWICE, w, 0, 1); loss = o.loss; }
+            if (DIST) { o = finish_row(a, teach_row(a, s, flags & SLOT_TWICE, 0, 1), Soft{zero, sum}, base, w); loss = o.loss; }
             else if (KIND != ROW_COEF) {
                 o = class_row<KIND>(a, Soft{zero, sum}, 0.0f, taken, w);
                 loss = o.loss; lp = o.lp;
@@ -768,7 +787,7 @@ __global__ void __launch_bounds__(TILE) k_row_tile(SoftArgs a, TileGeom ge) {
                         q = 0.0f;
                         for (int i = j; i < T; ++i) if (s.id[i] == s.id[j]) q += s.q[i];
                     }
-                    const float p = ex2(s.lp[j] * LOG2E);
+                    const float p = slot_p(a, o, s.z[j]);
                     z[s.id[j]] = w * a.tau * (o.mass * p - q);
                     if (a.h) h[s.id[j]] = o.hw * p * (1.0f - p);
                 }
@@ -910,10 +929,10 @@ __global__ void __launch_bounds__(TILE) k_row_few(SoftArgs a) {
     if (a.h) give(static_cast<float *>(a.h) + row0 * a.ldh, a.ldh, s_tile + TILE * K);
 }
 
-// What the CTAs of a cluster tell one another: maximum, sum and flags of their parts of a row.  Each writes its words into the shared memory
+// What the CTAs of a cluster tell one another: maximum and sum of their parts of a row.  Each writes its words into the shared memory
 // of all; a barrier there counts the bytes.
 struct Mail {
-    uint4 word[8];
+    float2 word[8];
     unsigned long long bar;
 };
 __device__ __forceinline__ uint32_t smem_at(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -921,12 +940,12 @@ __device__ __forceinline__ void bar_init(unsigned long long *bar, int count) { a
 __device__ __forceinline__ void bar_expect(unsigned long long *bar, int bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(bar)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void mail_send(Mail *m, int from, int to, Soft r, int flags) {
+__device__ __forceinline__ void mail_send(Mail *m, int from, int to, Soft r) {
     uint32_t at, bar;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_at(&m->word[from])), "r"(to));
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_at(&m->bar)), "r"(to));
-    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at), "r"(__float_as_uint(r.m)),
-                 "r"(__float_as_uint(r.s)), "r"(flags), "r"(0), "r"(bar) : "memory");
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(at), "r"(__float_as_uint(r.m)),
+                 "r"(__float_as_uint(r.s)), "r"(bar) : "memory");
 }
 // waits for a phase of a barrier, about a microsecond a try; false: it did not come within a second
 __device__ __forceinline__ bool bar_wait(unsigned long long *bar, unsigned parity) {
@@ -939,8 +958,21 @@ __device__ __forceinline__ bool bar_wait(unsigned long long *bar, unsigned parit
     return false;
 }
 
+// Whether a class has several slots: the classes go into an open table of at least twice as many places
+__host__ __device__ constexpr int table_places(int T) { int n = 64; while (n < 2 * T) n *= 2; return n; }
+__device__ __forceinline__ bool table_has(int *table, int places, int id) {
+    uint32_t at = (uint32_t)id * 2654435761u >> 16 & (places - 1);
+    for (int tries = 0; tries < places; ++tries) {
+        const int old = atomicCAS(table + at, -1, id);
+        if (old == -1) return false;
+        if (old == id) return true;
+        at = (at + 1) & (places - 1);
+    }
+    return false;
+}
+
 // One row for a CTA of NT threads, or for a cluster of 1 << lcs of them, up to V granules a thread.
-template <typename ZT, int KIND, int V, int NT>
+template <typename ZT, int KIND, int V, int NT, bool PRE = false>
 __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs, int words) {
     extern __shared__ __align__(16) unsigned char s_raw[];
     __shared__ Mail s_mail[2];
@@ -958,7 +990,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
     float w = KIND == ROW_COEF ? a.coef[row] : a.w ? a.w[row * a.w_stride] : 1.0f;
     if (CS > 1 && KIND != ROW_COEF) {
         if (t == 0) {
-            for (int q = 0; q < 2; ++q) { bar_init(&s_mail[q].bar, 1); bar_expect(&s_mail[q].bar, 16 * CS); }
+            for (int q = 0; q < 2; ++q) { bar_init(&s_mail[q].bar, 1); bar_expect(&s_mail[q].bar, 8 * CS); }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncthreads();
@@ -968,8 +1000,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
     const int count = at.ve - at.vs, left = count - t; // whole granules; of them, this thread's and those behind them
     const int end = t < at.ends ? at.end_at(t) : -1; // as many as threads at most
     const Slots s(s_raw, DIST ? a.T : 0);
-    uint32_t *bits = reinterpret_cast<uint32_t *>(s_raw + (size_t)a.T * Slots::BYTES);
-    bool live = w != 0.0f && (DIST || id != 0u);
+    uint32_t *bits = reinterpret_cast<uint32_t *>(s_raw + (PRE ? 0 : (size_t)a.T * Slots::BYTES));
+    TaughtRow pre = {};
+    if (DIST && PRE) pre.flags = __ldg(&a.taught[row].flags);
+    bool live = w != 0.0f && (DIST ? !PRE || (pre.flags & SLOT_SOME) : id != 0u);
     uint4 r[V];
     ZT end_raw = from_f<ZT>(-INFINITY);
     {
@@ -984,7 +1018,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
     }
     // what the class taken brings along, raw: a conversion here would wait for it
     const int code = DIST ? -1 : (int)id - 1;
-    int flags = live && !DIST && id > (uint32_t)a.K ? SLOT_BAD : 0;
+    int flags = DIST ? pre.flags : live && id > (uint32_t)a.K ? SLOT_BAD : 0;
     ZT code_raw = from_f<ZT>(0.0f);
     Taken taken = {};
     float2 st = make_float2(0.0f, 0.0f);
@@ -998,11 +1032,35 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
             if (a.ref) taken.ref = a.ref[i];
         }
     }
-    if (DIST && live) {
+    Teach teach = {};
+    if (DIST && PRE) {
+        if (live && t < 32) {
+            const float4 *from = reinterpret_cast<const float4 *>(a.taught + row);
+            const float4 x = __ldg(from), y = __ldg(from + 1);
+            teach = {x.x, x.y, x.z, x.w, y.x};
+        }
+        if (live && a.tail) { // marks of the classes named
+            for (int i = t; i < words; i += NT) bits[i] = 0u;
+            __syncthreads();
+            for (int j = t; j < a.T; j += NT) {
+                const uint32_t k = __ldg(a.ids + row * a.ldt + j);
+                const int b = (int)k - 1 + at.off - at.v0 * E;
+                if (k != 0u && k <= (uint32_t)a.K && b >= 0 && b < (at.v1 - at.v0) * E && load_t(a.t, a.t_dtype, row * a.ldt + j) != -INFINITY)
+                    atomicOr(&bits[b >> 5], 1u << (b & 31));
+            }
+            __syncthreads();
+        }
+    } else if (DIST && live) {
+        int *table = reinterpret_cast<int *>(bits + words);
+        const int places = table_places(a.T);
         if (t == 0) s_flags = 0;
         for (int i = t; i < words; i += NT) bits[i] = 0u;
+        for (int i = t; i < places; i += NT) table[i] = -1;
         __syncthreads();
-        for (int j = t; j < a.T; j += NT) flags |= put_into(a, at, s, bits, row, j);
+        for (int j = t; j < a.T; j += NT) {
+            flags |= put_into(a, at, s, bits, row, j);
+            if (s.id[j] >= 0 && table_has(table, places, s.id[j])) flags |= SLOT_TWICE; // of all classes, where the marks are of this CTA's
+        }
         flags = __reduce_or_sync(FULL, flags);
         if (lane == 0 && flags) atomicOr(&s_flags, flags);
         __syncthreads();
@@ -1060,11 +1118,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
             const float2 p = lane < WARPS ? s_part[lane] : make_float2(-INFINITY, 0.0f);
             all = lanes_join(Soft{p.x, p.y}, a.c, 32);
             if (CS > 1) {
-                if (t < CS) mail_send(mail, rank, t, all, flags);
+                if (t < CS) mail_send(mail, rank, t, all);
                 const bool came = bar_wait(&mail->bar, 0u);
-                const uint4 q = lane < CS ? mail->word[lane] : make_uint4(0xff800000u, 0u, 0u, 0u);
-                all = lanes_join(Soft{__uint_as_float(q.x), __uint_as_float(q.y)}, a.c, 32);
-                if (DIST) flags |= __reduce_or_sync(FULL, q.z); // each sees its own classes twice
+                const float2 q = lane < CS ? mail->word[lane] : make_float2(-INFINITY, 0.0f);
+                all = lanes_join(Soft{q.x, q.y}, a.c, 32);
                 if (!came) all.s = NAN;
             }
             return all;
@@ -1079,9 +1136,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
         }
         if (t < 32) {
             taken.z = to_f(code_raw);
-            if (DIST) o = slots_row(a, s, all, shift, flags & SLOT_TWICE, w, lane, 32);
+            if (DIST) o = finish_row(a, PRE ? teach : teach_row(a, s, flags & SLOT_TWICE, lane, 32), all, shift, w);
             else o = class_row<KIND>(a, all, shift, taken, w);
-            if (t == 0) {
+            if (lane == 0) {
                 s_out = o;
                 if (rank == 0) {
                     if ((DIST || KIND == ROW_POLICY) && a.loss) a.loss[row] = o.loss;
@@ -1118,10 +1175,80 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_row_ctas(SoftArgs a, int lcs,
     }
     if (DIST) {
         __syncthreads();
-        for (int j = t; j < a.T; j += NT) {
-            const int k = s.id[j], v = (k + at.off) / E;
-            if (k >= 0 && v >= at.v0 && v < at.v1) put_slot(a, at, o, s, j, flags & SLOT_TWICE, w);
+        if (PRE) {
+            const float2 q = __ldg(reinterpret_cast<const float2 *>(&a.taught[row].tmax)); // the largest of its logits, 1 / sum
+            for (int j = t; j < a.T; j += NT) {
+                const uint32_t k = __ldg(a.ids + row * a.ldt + j);
+                const int v = ((int)k - 1 + at.off) / E;
+                if (k == 0u || v < at.v0 || v >= at.v1) continue;
+                const float x = load_t(a.t, a.t_dtype, row * a.ldt + j);
+                if (x == -INFINITY) continue;
+                float qk = ex2(a.tail ? x * LOG2E : (x - q.x) * a.c) * q.y;
+                if (flags & SLOT_TWICE) { // the first slot of a class writes for all of them
+                    bool again = false;
+                    qk = 0.0f;
+                    for (int i = 0; i < a.T; ++i) {
+                        const float y = load_t(a.t, a.t_dtype, row * a.ldt + i);
+                        if (a.ids[row * a.ldt + i] != k || y == -INFINITY) continue;
+                        again = again || i < j;
+                        qk += ex2(a.tail ? y * LOG2E : (y - q.x) * a.c) * q.y;
+                    }
+                    if (again) continue;
+                }
+                const float p = slot_p(a, o, to_f(at.z[k - 1]));
+                if (at.g) at.g[k - 1] = from_f<ZT>(w * a.tau * (o.mass * p - qk));
+                if (at.h) at.h[k - 1] = from_f<ZT>(o.hw * p * (1.0f - p));
+            }
+        } else {
+            for (int j = t; j < a.T; j += NT) {
+                const int k = s.id[j], v = (k + at.off) / E;
+                if (k >= 0 && v >= at.v0 && v < at.v1) put_slot(a, at, o, s, j, flags & SLOT_TWICE, w);
+            }
         }
+    }
+}
+
+// The teacher's side of rows that k_row_ctas works on next: a warp per row.
+template <typename ZT>
+__global__ void __launch_bounds__(256) k_row_taught(SoftArgs a, TaughtRow *to) {
+    extern __shared__ __align__(16) unsigned char s_raw[];
+    const int lane = threadIdx.x & 31, places = table_places(a.T);
+    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= a.n) return;
+    unsigned char *mine = s_raw + (size_t)(threadIdx.x >> 5) * (a.T * Slots::BYTES + places * 4);
+    const Slots s(mine, a.T);
+    int *table = reinterpret_cast<int *>(mine + (size_t)a.T * Slots::BYTES);
+    const ZT *z = static_cast<const ZT *>(a.z) + row * a.ldz;
+    const float w = a.w ? a.w[row * a.w_stride] : 1.0f;
+    for (int i = lane; i < places; i += 32) table[i] = -1;
+    __syncwarp();
+    int flags = 0;
+    float tmax = -INFINITY;
+    for (int j = lane; j < a.T && w != 0.0f; j += 32) {
+        const uint32_t k = __ldg(a.ids + row * a.ldt + j);
+        const float t = load_t(a.t, a.t_dtype, row * a.ldt + j);
+        const bool use = k != 0u && t != -INFINITY, ok = use && k <= (uint32_t)a.K;
+        flags |= (use ? SLOT_SOME : 0) | (use && !ok ? SLOT_BAD : 0) | (ok && table_has(table, places, (int)k - 1) ? SLOT_TWICE : 0);
+        s.id[j] = ok ? (int)k - 1 : -1;
+        s.t[j] = t;
+        s.z[j] = ok ? to_f(z[k - 1]) : 0.0f;
+        if (ok) tmax = fmaxf(tmax, t);
+    }
+    flags = __reduce_or_sync(FULL, flags);
+    tmax = lanes_max(tmax, 32);
+    __syncwarp();
+    TaughtRow o = {};
+    o.flags = flags;
+    if ((flags & SLOT_SOME) && !(flags & SLOT_BAD)) {
+        o.teach = teach_row(a, s, flags & SLOT_TWICE, lane, 32);
+        float sum = 0.0f; // as teach_row has it
+        if (!a.tail) for (int j = lane; j < a.T; j += 32) if (s.id[j] >= 0) sum += ex2((s.t[j] - tmax) * a.inv_tau * LOG2E);
+        o.tmax = tmax;
+        o.r = a.tail ? 1.0f : 1.0f / lanes_sum(sum, 32);
+    }
+    if (lane == 0) {
+        if (!(flags & SLOT_SOME) || (flags & SLOT_BAD)) o.teach = Teach{};
+        to[row] = o;
     }
 }
 
@@ -1204,7 +1331,7 @@ __global__ void __launch_bounds__(512) k_row_walk(SoftArgs a, int words) {
         }
         if (KIND == ROW_DISTILL) {
             if (tid < 32) {
-                o = slots_row(a, s, all, shift, flags & SLOT_TWICE, w, lane, 32);
+                o = finish_row(a, teach_row(a, s, flags & SLOT_TWICE, lane, 32), all, shift, w);
                 if (tid == 0) s_out = o;
             }
             __syncthreads();
@@ -1288,7 +1415,7 @@ __global__ void __launch_bounds__(256) k_pairs(PairArgs a) {
 }
 
 // What may be resident at a time, asked once for every shape of a kernel
-constexpr int LANES_SMEM = 200 * 1024, WALK_SMEM = 160 * 1024, TILE_SMEM = 128 * 1024; // the attribute is set to the most a kernel is given: calls of several threads do not undo one another's
+constexpr int LANES_SMEM = 200 * 1024, WALK_SMEM = 160 * 1024, TILE_SMEM = 128 * 1024, TAUGHT_SMEM = 200 * 1024; // the attribute is set to the most a kernel is given: calls of several threads do not undo one another's
 cudaError_t launch_cluster(void (*kern)(SoftArgs, int, int), long long rows, int threads, int lcs, size_t smem, cudaStream_t st, const SoftArgs &a, int words) {
     cudaLaunchConfig_t c = {};
     cudaLaunchAttribute at[1];
@@ -1301,7 +1428,7 @@ cudaError_t launch_cluster(void (*kern)(SoftArgs, int, int), long long rows, int
     return cudaLaunchKernelEx(&c, kern, a, lcs, words);
 }
 template <typename ZT, int KIND>
-int32_t launch_typed(const SoftArgs &a, int sms, cudaStream_t st) {
+int32_t launch_typed(SoftArgs a, int sms, cudaStream_t st, void *work) {
     constexpr int E = Pack<ZT>::E;
     // granules of a row: of one that begins just before the end of its first one, unless all rows begin where a granule does
     const bool aligned = (uintptr_t)a.z % 16 == 0 && (a.ldz % E == 0 || a.n == 1);
@@ -1329,7 +1456,7 @@ int32_t launch_typed(const SoftArgs &a, int sms, cudaStream_t st) {
         ge.Kp = a.K | 1; ge.Tp = a.T | 1;
         ge.by_K = (uint32_t)((0x100000000ull + a.K - 1) / a.K); // not used for 1
         ge.by_T = a.T > 0 ? (uint32_t)((0x100000000ull + a.T - 1) / a.T) : 0u;
-        const size_t smem = 4 * (size_t)TILE * (ge.Kp * (a.h ? 2 : 1) + (KIND == ROW_DISTILL ? 5 * ge.Tp : 0));
+        const size_t smem = 4 * (size_t)TILE * (ge.Kp * (a.h ? 2 : 1) + (KIND == ROW_DISTILL ? 4 * ge.Tp : 0));
         if (smem > 47 * 1024) EVB_CUDA(cudaFuncSetAttribute(k_row_tile<ZT, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE_SMEM));
         EVB_CUDA(evb_launch(k_row_tile<ZT, KIND>, dim3((unsigned)((a.n + TILE - 1) / TILE)), dim3(TILE), smem, st, a, ge));
         return EVB_OK;
@@ -1354,7 +1481,8 @@ int32_t launch_typed(const SoftArgs &a, int sms, cudaStream_t st) {
     auto per = [&] { return (nvec + (1 << lcs) - 1) >> lcs; };
     auto holds = [&](int threads, int V) { return per() <= threads * V + (threads - 2 * E) / E; }; // the last few as ends, an element a thread
     auto go = [&](void (*kern)(SoftArgs, int, int), int threads) {
-        return launch_cluster(kern, a.n, threads, lcs, slots + (size_t)words_of(per()) * 4, st, a, words_of(per()));
+        const size_t smem = a.taught ? 0 : slots + (KIND == ROW_DISTILL ? (size_t)table_places(a.T) * 4 : 0);
+        return launch_cluster(kern, a.n, threads, lcs, smem + (size_t)words_of(per()) * 4, st, a, words_of(per()));
     };
     while (lcs < 3 && (a.n << (lcs + 1)) <= sms && per() > 256) ++lcs; // few rows: several SMs for each
     if (holds(1024, 2) && (a.n << lcs) <= 2 * sms) {
@@ -1364,6 +1492,17 @@ int32_t launch_typed(const SoftArgs &a, int sms, cudaStream_t st) {
     lcs = 0;
     while (lcs < 3 && !holds(256, 8)) ++lcs;
     if (holds(512, 8) && (a.n << lcs) <= 0x7fffffff) {
+        if constexpr (KIND == ROW_DISTILL) {
+            if (work) {
+                const size_t smem = 8 * (slots + (size_t)table_places(a.T) * 4);
+                if (smem > 47 * 1024) EVB_CUDA(cudaFuncSetAttribute(k_row_taught<ZT>, cudaFuncAttributeMaxDynamicSharedMemorySize, TAUGHT_SMEM));
+                EVB_CUDA(evb_launch(k_row_taught<ZT>, dim3((unsigned)((a.n + 7) / 8)), dim3(256), smem, st, a, static_cast<TaughtRow *>(work)));
+                a.taught = static_cast<const TaughtRow *>(work);
+                EVB_CUDA(holds(64, 8) ? go(k_row_ctas<ZT, KIND, 8, 64, true>, 64) : holds(128, 8) ? go(k_row_ctas<ZT, KIND, 8, 128, true>, 128)
+                         : holds(256, 8) ? go(k_row_ctas<ZT, KIND, 8, 256, true>, 256) : go(k_row_ctas<ZT, KIND, 8, 512, true>, 512));
+                return EVB_OK;
+            }
+        }
         EVB_CUDA(holds(64, 8) ? go(k_row_ctas<ZT, KIND, 8, 64>, 64) : holds(128, 8) ? go(k_row_ctas<ZT, KIND, 8, 128>, 128)
                  : holds(256, 8) ? go(k_row_ctas<ZT, KIND, 8, 256>, 256) : go(k_row_ctas<ZT, KIND, 8, 512>, 512));
         return EVB_OK;
@@ -1375,11 +1514,11 @@ int32_t launch_typed(const SoftArgs &a, int sms, cudaStream_t st) {
     return EVB_OK;
 }
 template <int KIND>
-int32_t launch_rows(const SoftArgs &a, int dtype, int device, cudaStream_t st) {
+int32_t launch_rows(const SoftArgs &a, int dtype, int device, cudaStream_t st, void *work = nullptr) {
     int sms = 0;
     EVB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
-    return dtype == EVB_BF16 ? launch_typed<__nv_bfloat16, KIND>(a, sms, st) : dtype == EVB_F16 ? launch_typed<__half, KIND>(a, sms, st)
-                                                                                                : launch_typed<float, KIND>(a, sms, st);
+    return dtype == EVB_BF16 ? launch_typed<__nv_bfloat16, KIND>(a, sms, st, work) : dtype == EVB_F16 ? launch_typed<__half, KIND>(a, sms, st, work)
+                                                                                                : launch_typed<float, KIND>(a, sms, st, work);
 }
 
 // the calling thread's device is what it was when the call returns
@@ -1484,18 +1623,19 @@ int32_t evb_launch_objective(evb_handle *h, bool eval) {
 
 extern "C" int32_t evb_distill_grads(int32_t device, void *stream, const void *z, int32_t dtype, int64_t n, int32_t K, int64_t ldz, const uint32_t *ids,
                                      const void *teacher, int32_t teacher_dtype, int32_t T, int32_t tail, const float *w, double tau, float *loss,
-                                     void *grad, int64_t ldg, void *hess, int64_t ldh) {
+                                     void *grad, int64_t ldg, void *hess, int64_t ldh, void *work) {
     EVB_CHECK(check_rows("evb_distill_grads", z, dtype, n, K, ldz, grad, ldg, hess, ldh));
     if (T < 1 || !known_dtype(teacher_dtype)) { evb_set_error("evb_distill_grads: a row has at least one slot, of EVB_F32, EVB_BF16 or EVB_F16"); return EVB_ERR_ARG; }
     if (T > MAX_TOP) { evb_set_error("evb_distill_grads: %d slots, the limit is %d", T, MAX_TOP); return EVB_ERR_LIMIT; }
     if (!good_tau(tau) || (tail && tau != 1.0)) { evb_set_error("evb_distill_grads: tau must lie in [1e-6, 1e6], and be 1 with a tail (tau = %g)", tau); return EVB_ERR_ARG; }
     if (n > 0 && (!ids || !teacher)) { evb_set_error("evb_distill_grads: null pointer"); return EVB_ERR_ARG; }
+    if ((uintptr_t)work % 16) { evb_set_error("evb_distill_grads: misaligned pointer"); return EVB_ERR_ARG; }
     OnDevice dev;
     EVB_CHECK(dev.enter("evb_distill_grads", device));
     if (n == 0) return EVB_OK;
     SoftArgs a = rows_args(z, n, K, ldz, w, (float)tau, loss, grad, ldg, hess, ldh);
     a.ids = ids; a.t = teacher; a.t_dtype = teacher_dtype; a.T = T; a.ldt = T; a.tail = tail != 0;
-    return launch_rows<ROW_DISTILL>(a, dtype, device, (cudaStream_t)stream);
+    return launch_rows<ROW_DISTILL>(a, dtype, device, (cudaStream_t)stream, work);
 }
 
 extern "C" int32_t evb_policy_grads(int32_t device, void *stream, const void *z, int32_t dtype, int64_t n, int32_t K, int64_t ldz, const uint32_t *action,

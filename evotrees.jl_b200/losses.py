@@ -73,8 +73,9 @@ def distill_grads(pred, ids, teacher, *, w=None, tau: float = 1.0, tail: bool = 
     pw = None if w is None else _vec("w", w, (n,), _F32, dev)
     loss = torch.empty(n, dtype=_F32, device=dev)
     g, pg, h, ph = _outputs(pred, n, K, grads, hess)
+    work = torch.empty(8 * n, dtype=_F32, device=dev) if K > 1000 else None
     rc = _lib.lib().evb_distill_grads(dev.index, _lib.raw_stream(dev.index), pred.data_ptr(), code, n, K, ld, pi, pt, tcode, T, bool(tail), pw, tau,
-                                      loss.data_ptr(), pg, K, ph, K)
+                                      loss.data_ptr(), pg, K, ph, K, None if work is None else work.data_ptr())
     if rc:
         _lib.check(rc)
     return (loss,) if g is None else (loss, g) if h is None else (loss, g, h)

@@ -417,6 +417,8 @@ EVB_API int32_t evb_hist_rows_noalloc(int32_t device, void *stream, const uint8_
  * evb_distill_grads -- Kullback-Leibler divergence from a teacher of whom T classes a row were kept.
  *   ids      device uint32 [n][T] class codes, 0 = empty slot;  teacher  device [n][T], own type; a slot that holds -inf is empty too.
  *            1 <= T <= 1024.  Rows without slots count for nothing.  A class in several slots counts with each of them.
+ *   work     device, 32 n bytes, 16-byte aligned, in use until the call's kernels are done; or NULL.  Many rows of more than 4 KB take a
+ *            launch before the others for the teacher's side when there is room for what it finds
  *   tail=0   teacher holds logits: q_j = e^(t_j / tau) / sum, over the slots
  *            loss = w tau^2 sum_j q_j (log q_j - log p_j),  grad_k = w tau (p_k - sum of q_j of class k)
  *   tail=1   (tau = 1) teacher holds log-probabilities: q_j = e^t_j; the rest q_T = max(0, 1 - sum_j q_j) is compared with the
@@ -443,7 +445,7 @@ EVB_API int32_t evb_hist_rows_noalloc(int32_t device, void *stream, const uint8_
  */
 EVB_API int32_t evb_distill_grads(int32_t device, void *stream, const void *z, int32_t dtype, int64_t n, int32_t K, int64_t ldz, const uint32_t *ids,
                                   const void *teacher, int32_t teacher_dtype, int32_t T, int32_t tail, const float *w, double tau, float *loss,
-                                  void *grad, int64_t ldg, void *hess, int64_t ldh);
+                                  void *grad, int64_t ldg, void *hess, int64_t ldh, void *work);
 EVB_API int32_t evb_policy_grads(int32_t device, void *stream, const void *z, int32_t dtype, int64_t n, int32_t K, int64_t ldz, const uint32_t *action,
                                  const float *old_logp, const float *adv, const float *ref_logp, const float *w, double tau, double clip_low,
                                  double clip_high, double beta, float *loss, float *logp, void *grad, int64_t ldg, void *hess, int64_t ldh);

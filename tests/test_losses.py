@@ -8,7 +8,7 @@ Z = 4096    # an address that is never read
 
 
 def _distill(lib, **kw):
-    a = dict(device=0, stream=None, z=Z, dtype=0, n=4, K=5, ldz=5, ids=Z, t=Z, tdtype=0, T=2, tail=0, w=None, tau=1.0, loss=Z, g=Z, ldg=5, h=None, ldh=5)
+    a = dict(device=0, stream=None, z=Z, dtype=0, n=4, K=5, ldz=5, ids=Z, t=Z, tdtype=0, T=2, tail=0, w=None, tau=1.0, loss=Z, g=Z, ldg=5, h=None, ldh=5, work=None)
     a.update(kw)
     return lib.evb_distill_grads(*a.values())
 
@@ -33,7 +33,7 @@ ROWS = [dict(dtype=1), dict(dtype=2), dict(dtype=9), dict(n=-1), dict(n=2_000_00
 
 
 @pytest.mark.parametrize("kw", ROWS + [dict(T=0), dict(tdtype=1), dict(tau=0.0), dict(tau=-1.0), dict(tau=NAN), dict(tau=float("inf")), dict(tail=1, tau=2.0),
-                                       dict(ids=None), dict(t=None), dict(h=Z, ldh=4), dict(h=Z + 2)])
+                                       dict(ids=None), dict(t=None), dict(h=Z, ldh=4), dict(h=Z + 2), dict(work=Z + 8)])
 def test_distill_refuses(pkg, kw):
     from evotrees_b200 import _lib
     assert _distill(_lib.lib(), **kw) == -1 and b"evb_distill_grads" in _lib.lib().evb_last_error()

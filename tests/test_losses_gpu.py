@@ -73,6 +73,33 @@ def test_distill_sizes(pkg, K, dtype):
     check_distill(out, z, ids, lt, None, 1.0, True, hess)
 
 
+@pytest.mark.parametrize("K", [2500, 20011, 70001, 200003])
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_with_and_without_work_memory(pkg, K, tail):
+    """Enough rows for a launch of its own for the teacher's side, which the C entry leaves out without work memory."""
+    from evotrees_b200 import _lib
+    rng = np.random.default_rng(K)
+    n, T = 320, 70
+    z, zd = logits(rng, n, K, torch.bfloat16)
+    ids, t = slots(rng, n, K, T)
+    ids[5] = 0
+    ids[7, 3] = K + 1
+    ids[9, :6] = ids[9, 0].clamp(min=1)                            # a class again and again
+    w = torch.ones(n)
+    w[11] = 0.0
+    t = log_probs(t, 0.9) if tail else t
+    idd, td, wd = ids.cuda(), t.cuda(), w.cuda()
+    loss, g = pkg.distill_grads(zd, idd, td, w=wd, tail=tail)
+    loss2, g2 = torch.empty(n, device="cuda"), torch.empty_like(g)
+    _lib.check(_lib.lib().evb_distill_grads(0, 0, zd.data_ptr(), _lib.EVB_BF16, n, K, K, idd.data_ptr(), td.data_ptr(), _lib.EVB_F32, T, int(tail), wd.data_ptr(),
+                                            1.0, loss2.data_ptr(), g2.data_ptr(), K, None, 0, None))
+    torch.cuda.synchronize()
+    keep = [0, 1, 5, 9, 11, n - 1]
+    for out in ((loss, g), (loss2, g2)):
+        assert torch.isnan(out[0][7]) and torch.isnan(out[1][7]).all()
+        check_distill([o[keep] for o in out], z[keep], ids[keep], t[keep], w[keep], 1.0, tail, False)
+
+
 @pytest.mark.parametrize("K,T", [(40, 40), (40, 39), (1500, 1024), (9000, 700), (131072, 1024), (7, 1)])
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_many_slots(pkg, K, T, tail):
@@ -365,7 +392,7 @@ def test_output_strides_write_nothing_else(pkg, K, dtype):
         loss = torch.empty(n, device="cuda")
         idd, td = ids.cuda(), t.cuda()
         _lib.check(_lib.lib().evb_distill_grads(0, 0, zd.data_ptr(), _lib.EVB_F32 if dtype == "f32" else _lib.EVB_BF16, n, K, K, idd.data_ptr(), td.data_ptr(),
-                                                _lib.EVB_F32, t.shape[1], 0, None, 1.0, loss.data_ptr(), g[off:].data_ptr(), ld, h[off:].data_ptr(), ld))
+                                                _lib.EVB_F32, t.shape[1], 0, None, 1.0, loss.data_ptr(), g[off:].data_ptr(), ld, h[off:].data_ptr(), ld, None))
         torch.cuda.synchronize()
         for buf, w, mark in ((g, want[1], 77.0), (h, want[2], 78.0)):
             body = buf[off:off + n * ld].view(n, ld)
