@@ -3,6 +3,14 @@
 //
 // All three need the same of a row z[0 .. K-1]: its maximum and the sum of 2^(c (z_k - max)), c = log2(e) / tau, a few named columns,
 // and then one number A so that g_k = A 2^(c (z_k - max)) everywhere but at the named columns, which are written after the others.
+// What bounds them is memory: a row is read once and its gradient written once (twice with hessians); a preference reads its rows a second time,
+// because a row's factor depends on all rows of its pair.  Which kernel takes a row is a matter of its size (launch_typed):
+//   k_row_few    2 to 8 classes of 32 bits: a thread per row, in registers
+//   k_row_tile   up to 32 classes and slots: a thread per row, staged through shared memory
+//   k_row_lanes  up to 256 granules of 16 bytes (1024 floats): some lanes of a warp
+//   k_row_ctas   up to 32768 granules: a CTA, or a cluster of up to eight; with two granules a thread where there are few rows
+//   k_row_walk   beyond: a CTA reads the row twice
+// Sums, maxima, probabilities and losses are 32-bit floats, sums of log ratios 64-bit ones; the only rounding to 16 bits is that of the results.
 #include "evb_device.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -475,7 +483,10 @@ __device__ __forceinline__ RowOut class_row(const SoftArgs &a, Soft r, float shi
     o.M = base_of(r.m, a.c);
     o.shift = shift;
     o.B = 1.0f / r.s;
-    o.lp = LN2 * (fmaf(t.z - shift, a.c, -o.M) - log2f(r.s));
+    // A preference adds up hundreds of them: 64 bits, and in units of the c that the terms were made with, so that roundings which all rows share
+    // do not add up too
+    if (KIND == ROW_LOGP) o.lp = (float)((fma((double)(t.z - shift), (double)a.c, -(double)o.M) - log2((double)r.s)) / ((double)a.c * (double)a.tau));
+    else o.lp = LN2 * (fmaf(t.z - shift, a.c, -o.M) - log2f(r.s));
     o.mass = 0.0f;
     o.loss = 0.0f;
     if (KIND == ROW_POLICY) {
@@ -576,6 +587,8 @@ __device__ __forceinline__ int put_into(const SoftArgs &a, const RowAt<ZT> &at, 
 
 // Rows of up to V granules for each of G lanes (a power of two up to 32): 32 / G rows a warp, 8 warps a CTA.
 template <typename ZT, int KIND, int V>
+// The row stays in registers between its two uses.  Measured: policy 20011 x 1000 f32 34 us (floor 24), 100k x 200 f32 with ten slots 65 (26): there
+// most instructions are the slots' (12000 of a row's threads together, of which the 200 classes take 2000).
 __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words) {
     extern __shared__ __align__(16) unsigned char s_raw[];
     constexpr int E = Pack<ZT>::E;
@@ -656,6 +669,7 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
 
 // Rows of up to 32 classes: a thread per row, 128 rows a CTA, all that they hold staged through shared memory so that memory is read and written
 // in order.  Rows of shared memory are an odd number of words apart: neighbours fall into different banks.
+// Policy 1M x 18 with hessians: 52 us (floor 37).
 constexpr int TILE = 128, TILE_K = 32, TILE_T = 32;
 struct TileGeom { int Kp, Tp; uint32_t by_K, by_T; }; // by_*: (c * by) >> 32 is c / K (c / T) for c < 2^13
 template <typename T, typename F>
@@ -805,6 +819,7 @@ __global__ void __launch_bounds__(TILE) k_row_tile(SoftArgs a, TileGeom ge) {
 
 // The same for 2 to 8 classes of 32 bits, their number known to the compiler: a row's predictions stay in registers, read by their thread alone (the
 // rows of a warp are neighbours: what one thread leaves of a line, others take); gradients and hessians go out through shared memory.
+// 2M x 5 with three slots and hessians: 65 us (floor 28); k_row_tile takes 100, 1400 instructions a row.
 template <int KIND, int K>
 __global__ void __launch_bounds__(TILE) k_row_few(SoftArgs a) {
     extern __shared__ __align__(16) float s_tile[]; // gradients [TILE][K], hessians
@@ -971,7 +986,13 @@ __device__ __forceinline__ bool table_has(int *table, int places, int id) {
     return false;
 }
 
-// One row for a CTA of NT threads, or for a cluster of 1 << lcs of them, up to V granules a thread.
+// One row for a CTA of NT threads, or for a cluster of 1 << lcs of them, up to V granules a thread.  The row stays in registers (16-bit predictions
+// packed, their exponentials worked out twice; 32-bit ones as their terms), so it is read once.  Between loads and stores lies a chain that
+// no single row can hide (the sums over lanes, warps, CTAs; the row's numbers: some 4000 of 12000 clocks), so what counts is how many rows an SM has
+// in hand: eight granules a thread at 64 registers, 1024 threads.  Measured and left: rows that a CTA stays for, fetched ahead by bulk
+// copies into a ring (2.4 to 3.0 TB/s instead of 4.2); independent warps in two passes, the second out of L2 (2.1); a warp more for the slots
+// (three CTAs an SM instead of four: 770 us instead of 597).  4.9 TB/s for 8192 x 65537 bf16 (420 us, floor 316).
+// PRE: k_row_taught has seen to the slots (4096 x 131072 bf16 with 64 and a tail: 523 us, floor 322; 597 without).
 template <typename ZT, int KIND, int V, int NT, bool PRE = false>
 __global__ void __launch_bounds__(NT, (V == 16 ? 512 : 1024) / NT) k_row_ctas(SoftArgs a, int lcs, int words) {
     extern __shared__ __align__(16) unsigned char s_raw[];
