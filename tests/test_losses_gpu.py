@@ -100,6 +100,54 @@ def test_distill_with_and_without_work_memory(pkg, K, tail):
         check_distill([o[keep] for o in out], z[keep], ids[keep], t[keep], w[keep], 1.0, tail, False)
 
 
+def test_distill_most_slots_of_many_rows_in_a_graph(pkg):
+    rng = np.random.default_rng(8)
+    n, K, T = 300, 5000, 1024
+    z, zd = logits(rng, n, K, torch.float32)
+    ids, t = slots(rng, n, K, T)
+    lt = log_probs(t, 0.9)
+    idd, td = ids.cuda(), lt.cuda()
+    plain = pkg.distill_grads(zd, idd, td, tail=True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = pkg.distill_grads(zd, idd, td, tail=True)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(plain, out))
+    keep = [0, 150, n - 1]
+    check_distill([o[keep] for o in out], z[keep], ids[keep], lt[keep], None, 1.0, True, False)
+
+
+def test_calls_of_several_threads(pkg):
+    """Calls of different sizes at the same time, each thread on its own stream: the bits of calls one by one."""
+    import threading
+    rng = np.random.default_rng(12)
+    jobs = []
+    for n, K, T in ((300, 5, 3), (200, 300, 40), (320, 9000, 70), (12, 40000, 5)):
+        z, zd = logits(rng, n, K, torch.float32)
+        ids, t = slots(rng, n, K, T) if T <= K else None
+        jobs.append((zd, ids.cuda(), t.cuda()))
+    torch.cuda.synchronize()
+    want = [pkg.distill_grads(*j) for j in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(j, w):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                out = pkg.distill_grads(*j)
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(x, y) for x, y in zip(out, w)):
+                    wrong.append(j[0].shape)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(jobs, want)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
+
+
 @pytest.mark.parametrize("K,T", [(40, 40), (40, 39), (1500, 1024), (9000, 700), (131072, 1024), (7, 1)])
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_many_slots(pkg, K, T, tail):
