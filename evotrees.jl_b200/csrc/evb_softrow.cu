@@ -443,7 +443,8 @@ __device__ __forceinline__ Teach teach_row(const SoftArgs &a, const Slots &s, bo
 // r: maximum and sum of the row, less `shift`; with a tail of the classes that have no slot
 __device__ __forceinline__ RowOut finish_row(const SoftArgs &a, const Teach &e, Soft r, float shift, float w) {
     const float c = a.c, zn = e.zn - shift;
-    const Soft all = a.tail ? join(Soft{zn, e.s}, r, c) : r;
+    // e.s is relative to c zn itself, a Soft to that rounded: they differ by up to half a step of the product, which is an exponent
+    const Soft all = a.tail ? join(Soft{zn, e.s * ex2(fmaf(zn, c, -base_of(zn, c)))}, r, c) : r;
     const float M = base_of(all.m, c), ls = log2f(all.s);
     // the rest, when there is any: no class is left where every one is named or ruled out
     const float qt = a.tail && r.m != -INFINITY ? fmaxf(0.0f, 1.0f - e.Q) : 0.0f;
