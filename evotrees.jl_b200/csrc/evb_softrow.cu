@@ -1320,11 +1320,11 @@ __global__ void __launch_bounds__(512) k_row_walk(SoftArgs a, int words) {
     RowOut o = {};
     float shift = 0.0f;
     RowAt<ZT> piece = at; // 4 granules a thread at a time, the ends with the last
+    const uint32_t *out = KIND == ROW_DISTILL && a.tail ? bits : nullptr;
     if (KIND == ROW_COEF) {
         o = coef_row(a, a.stat[row], a.logp[row], w);
         shift = o.shift;
     } else {
-        const uint32_t *out = KIND == ROW_DISTILL && a.tail ? bits : nullptr;
         Soft all = {-INFINITY, 0.0f};
         for (piece.vs = at.vs; piece.vs < at.ve || piece.vs == at.vs; piece.vs += 4 * nt) {
             const bool last = piece.vs + 4 * nt >= at.ve;
@@ -1372,9 +1372,9 @@ __global__ void __launch_bounds__(512) k_row_walk(SoftArgs a, int words) {
         uint4 r[4];
         fetch<ZT, 4>(r, piece, tid, nt, true);
         float scale = 1.0f;
-        if (E == 4 && KIND != ROW_COEF) { // terms
-            if (shift != 0.0f) take_far<ZT, 4>(r, piece, shift, a.c, nullptr, tid, nt);
-            else scale = ex2(rise(take<ZT, 4>(r, piece, a.c, nullptr, tid, nt, false).m, a.c, o.M));
+        if (E == 4 && KIND != ROW_COEF) { // terms, of the classes that were summed: a named one far above them would be the maximum of its thread's
+            if (shift != 0.0f) take_far<ZT, 4>(r, piece, shift, a.c, out, tid, nt);
+            else scale = ex2(rise(take<ZT, 4>(r, piece, a.c, out, tid, nt, false).m, a.c, o.M));
         } else if (shift != 0.0f) less<ZT, 4>(r, piece, shift, nullptr, tid, nt);
         give<ZT, KIND, 4>(a, piece, o, r, tid, nt, scale, code);
     }

@@ -37,3 +37,16 @@ def test_offsets(pkg, K, offset):
     ids, t = slots(rng, n, K, min(64, K - 2), empty=0.0)
     t = log_probs(t, 0.7)
     check(pkg.distill_grads(z.cuda(), ids.cuda(), t.cuda(), tail=True, hess=True), z, ids, t, hess=True)
+
+
+@pytest.mark.parametrize("above", [100.0, 1.0e4])
+@pytest.mark.parametrize("K,dtype", [(1000, "f32"), (9000, "f32"), (70001, "f32"), (131073, "f32"), (200003, "f32"), (270001, "bf16")])
+def test_named_classes_above_all_others(pkg, K, dtype, above):
+    """The classes that the teacher names lie further above the others than 32-bit exponents reach."""
+    rng = np.random.default_rng(K)
+    n = 4
+    z, _ = logits(rng, n, K, DTYPES[dtype])
+    ids, t = slots(rng, n, K, 40, empty=0.0)
+    z.scatter_(1, ids.long() - 1, (above + torch.from_numpy(rng.normal(size=(n, 40)))).to(z.dtype))
+    t = log_probs(t, 0.9)
+    check(pkg.distill_grads(z.cuda(), ids.cuda(), t.cuda(), tail=True, hess=True), z, ids, t, hess=True)
