@@ -404,7 +404,8 @@ struct RowOut {
     float hw;           // hessian hw p (1 - p)
     float lp;           // log p of the class taken
     float loss;
-    float all_M, all_ls; // distillation: log2 of the sum over all classes, in two parts
+    float all_M, all_ls; // distillation: log2 of the sum over all classes, in two parts, ..
+    float all_shift;     // .. of predictions less this: 0, or their maximum
 };
 __device__ __forceinline__ bool first_slot(const Slots &s, int j) {
     for (int i = 0; i < j; ++i) if (s.id[i] == s.id[j]) return false;
@@ -440,31 +441,38 @@ __device__ __forceinline__ Teach teach_row(const SoftArgs &a, const Slots &s, bo
     o.Q = 1.0f;
     return o;
 }
-// r: maximum and sum of the row, less `shift`; with a tail of the classes that have no slot
+// r: maximum and sum of the row, less `shift`; with a tail of the classes that have no slot.  The named ones may lie anywhere then (masks leave
+// them alone, or only them): all classes together are relative to the larger of the two maxima, those without a slot among themselves to theirs.
 __device__ __forceinline__ RowOut finish_row(const SoftArgs &a, const Teach &e, Soft r, float shift, float w) {
-    const float c = a.c, zn = e.zn - shift;
-    // e.s is relative to c zn itself, a Soft to that rounded: they differ by up to half a step of the product, which is an exponent
-    const Soft all = a.tail ? join(Soft{zn, e.s * ex2(fmaf(zn, c, -base_of(zn, c)))}, r, c) : r;
-    const float M = base_of(all.m, c), ls = log2f(all.s);
-    // the rest, when there is any: no class is left where every one is named or ruled out
-    const float qt = a.tail && r.m != -INFINITY ? fmaxf(0.0f, 1.0f - e.Q) : 0.0f;
+    const float c = a.c, zn = e.zn, zr = r.m + shift;
+    const bool above = a.tail && zn > zr;
     RowOut o;
-    o.loss = e.H - LN2 * (e.qz + (zn == -INFINITY ? e.qz == 0.0f ? 0.0f : zn : (fmaf(zn, c, -M) - ls) * e.Q));
-    if (zn == -INFINITY && e.Q > 0.0f) o.loss = all.m == -INFINITY ? NAN : INFINITY; // nothing that the teacher names is possible
-    if (qt > 0.0f) o.loss += qt * (logf(qt) - LN2 * (rise(r.m, c, M) + log2f(r.s) - ls));
     o.M = base_of(r.m, c);
     o.shift = shift;
+    o.all_shift = !above ? shift : is_far(zn, c) ? zn : 0.0f;
+    o.all_M = !above ? o.M : base_of(zn - o.all_shift, c);
+    // The exponent that brings r.s there.  r.s is relative to c r.m rounded, e.s to c zn itself: they differ by up to half a step of the product
+    const float part = !above ? 0.0f : zr == -INFINITY ? zr : fmaf(zr - o.all_shift, c, -o.all_M) - fmaf(r.m, c, -o.M);
+    float sum = above ? r.s * ex2(part) : r.s;
+    if (a.tail) sum += e.s * ex2(fmaf(zn - o.all_shift, c, -o.all_M));
+    const float ls = o.all_ls = log2f(sum);
+    // the rest, when there is any: no class is left where every one is named or ruled out
+    const float qt = a.tail && r.m != -INFINITY ? fmaxf(0.0f, 1.0f - e.Q) : 0.0f;
+    o.loss = e.H - LN2 * (e.qz + (zn == -INFINITY ? e.qz == 0.0f ? 0.0f : zn : (fmaf(zn - o.all_shift, c, -o.all_M) - ls) * e.Q));
+    if (zn == -INFINITY && e.Q > 0.0f) o.loss = zr == -INFINITY ? NAN : INFINITY; // nothing that the teacher names is possible
+    if (qt > 0.0f) {
+        const float y = part + log2f(r.s) - ls; // a number of which the product with c overflows still has a logarithm
+        o.loss += qt * (logf(qt) - (y == -INFINITY ? zr - zn : LN2 * y));
+    }
     o.mass = e.Q + qt;
-    o.all_M = M;
-    o.all_ls = ls;
-    o.B = r.m == -INFINITY ? 0.0f * ls : ex2(rise(r.m, c, M)) / all.s;
+    o.B = r.m == -INFINITY ? 0.0f * ls : ex2(part) / sum;
     o.A = w * a.tau * (o.mass * o.B - (qt > 0.0f ? qt / r.s : 0.0f));
     o.hw = w;
     o.special = o.lp = 0.0f;
     o.loss *= w * a.tau * a.tau;
     return o;
 }
-__device__ __forceinline__ float slot_p(const SoftArgs &a, const RowOut &o, float z) { return ex2(fmaf(z - o.shift, a.c, -o.all_M) - o.all_ls); }
+__device__ __forceinline__ float slot_p(const SoftArgs &a, const RowOut &o, float z) { return ex2(fmaf(z - o.all_shift, a.c, -o.all_M) - o.all_ls); }
 __device__ __forceinline__ float less_p(float lp) { return lp < -0.5f ? 1.0f - ex2(lp * LOG2E) : -expm1f(lp); } // 1 - p, also where p is close to 1
 // what belongs to the class taken, read ahead of its use
 struct Taken { float z, old_lp, adv, ref; };
@@ -893,7 +901,7 @@ __global__ void __launch_bounds__(TILE) k_row_few(SoftArgs a) {
 #pragma unroll
                     for (int k = 0; k < K; ++k) if (!(out >> k & 1u)) rest += ex2((z[k] - rbase) * c);
                     rr = qt / rest;
-                    if (qt > 0.0f) loss += qt * (logf(qt) - LN2 * ((rbase - base) * c + log2f(rest) - ls));
+                    if (qt > 0.0f) loss += qt * (logf(qt) - (rbase - base) - LN2 * (log2f(rest) - ls)); // tau = 1
                 }
                 const float mass = a.tail ? Q + qt : 1.0f, f = w * a.tau;
 #pragma unroll
