@@ -412,7 +412,7 @@ __device__ __forceinline__ bool first_slot(const Slots &s, int j) {
     return true;
 }
 // What a row's slots say by themselves, before its maximum and sum are known: the sum Q of the teacher's probabilities (1 without a tail), sum q log q,
-// the largest named prediction zn, sum q c (z - zn), and (tail) sum of 2^(c (z - zn)) over the classes named, each of them once
+// the largest named prediction zn, sum q (z - zn) / tau, and (tail) sum of 2^(c (z - zn)) over the classes named, each of them once
 struct Teach { float Q, H, zn, qz, s; };
 struct alignas(16) TaughtRow { Teach teach; int flags; float tmax, r; }; // slots' flags; their largest logit, 1 / sum
 // `width` lanes share the slots; all of them get the same.  Slots without a class have id -1
@@ -426,11 +426,11 @@ __device__ __forceinline__ Teach teach_row(const SoftArgs &a, const Slots &s, bo
     const float zn = o.zn == -INFINITY ? 0.0f : o.zn;
     for (int j = lane; j < a.T; j += width) {
         if (s.id[j] < 0) continue;
-        const float lt = a.tail ? s.t[j] : (s.t[j] - tmax) * a.inv_tau, e = ex2(lt * LOG2E), d = (s.z[j] - zn) * c;
+        const float lt = a.tail ? s.t[j] : (s.t[j] - tmax) * a.inv_tau, e = ex2(lt * LOG2E), d = s.z[j] - zn;
         s.q[j] = e;
         o.Q += e;
-        if (e != 0.0f) { o.H += e * lt; o.qz += e * d; }
-        if (a.tail && (!dup || first_slot(s, j))) o.s += ex2(d);
+        if (e != 0.0f) { o.H += e * lt; o.qz += e * (d * a.inv_tau); }
+        if (a.tail && (!dup || first_slot(s, j))) o.s += ex2(d * c);
     }
     o.Q = lanes_sum(o.Q, width); o.H = lanes_sum(o.H, width); o.qz = lanes_sum(o.qz, width);
     if (a.tail) { o.s = lanes_sum(o.s, width); return o; }
@@ -441,6 +441,8 @@ __device__ __forceinline__ Teach teach_row(const SoftArgs &a, const Slots &s, bo
     o.Q = 1.0f;
     return o;
 }
+// log p = y ln 2, from the difference to the row's maximum where the product with c, not that itself, is beyond 32 bits
+__device__ __forceinline__ float log_p(const SoftArgs &a, float y, float less_max) { return y == -INFINITY ? less_max * a.inv_tau : LN2 * y; }
 // r: maximum and sum of the row, less `shift`; with a tail of the classes that have no slot.  The named ones may lie anywhere then (masks leave
 // them alone, or only them): all classes together are relative to the larger of the two maxima, those without a slot among themselves to theirs.
 __device__ __forceinline__ RowOut finish_row(const SoftArgs &a, const Teach &e, Soft r, float shift, float w) {
@@ -458,12 +460,10 @@ __device__ __forceinline__ RowOut finish_row(const SoftArgs &a, const Teach &e, 
     const float ls = o.all_ls = log2f(sum);
     // the rest, when there is any: no class is left where every one is named or ruled out
     const float qt = a.tail && r.m != -INFINITY ? fmaxf(0.0f, 1.0f - e.Q) : 0.0f;
-    o.loss = e.H - LN2 * (e.qz + (zn == -INFINITY ? e.qz == 0.0f ? 0.0f : zn : (fmaf(zn - o.all_shift, c, -o.all_M) - ls) * e.Q));
+    const float lp = log_p(a, fmaf(zn - o.all_shift, c, -o.all_M) - ls, zn - (above ? zn : zr));
+    o.loss = e.H - (e.qz + (zn == -INFINITY ? e.qz == 0.0f ? 0.0f : zn : e.Q > 0.0f ? lp * e.Q : 0.0f));
     if (zn == -INFINITY && e.Q > 0.0f) o.loss = zr == -INFINITY ? NAN : INFINITY; // nothing that the teacher names is possible
-    if (qt > 0.0f) {
-        const float y = part + log2f(r.s) - ls; // a number of which the product with c overflows still has a logarithm
-        o.loss += qt * (logf(qt) - (y == -INFINITY ? zr - zn : LN2 * y));
-    }
+    if (qt > 0.0f) o.loss += qt * (logf(qt) - log_p(a, part + log2f(r.s) - ls, zr - (above ? zn : zr)));
     o.mass = e.Q + qt;
     o.B = r.m == -INFINITY ? 0.0f * ls : ex2(part) / sum;
     o.A = w * a.tau * (o.mass * o.B - (qt > 0.0f ? qt / r.s : 0.0f));
@@ -495,7 +495,7 @@ __device__ __forceinline__ RowOut class_row(const SoftArgs &a, Soft r, float shi
     // A preference adds up hundreds of them: 64 bits, and in units of the c that the terms were made with, so that roundings which all rows share
     // do not add up too
     if (KIND == ROW_LOGP) o.lp = (float)((fma((double)(t.z - shift), (double)a.c, -(double)o.M) - log2((double)r.s)) / ((double)a.c * (double)a.tau));
-    else o.lp = LN2 * (fmaf(t.z - shift, a.c, -o.M) - log2f(r.s));
+    else o.lp = log_p(a, fmaf(t.z - shift, a.c, -o.M) - log2f(r.s), t.z - shift - r.m);
     o.mass = 0.0f;
     o.loss = 0.0f;
     if (KIND == ROW_POLICY) {
@@ -907,7 +907,7 @@ __global__ void __launch_bounds__(TILE) k_row_few(SoftArgs a) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     const float qk = q[k] * rQ, p = y[k] * r;
-                    if (qk != 0.0f) loss -= qk * (LN2 * ((z[k] - base) * c - ls));
+                    if (qk != 0.0f) loss -= qk * ((z[k] - base) * a.inv_tau - LN2 * ls);
                     float g = mass * p - qk;
                     if (a.tail && !(out >> k & 1u) && qt > 0.0f) g = mass * p - rr * ex2((z[k] - rbase) * c);
                     z[k] = f * g;

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests import losses_ref as R
-from tests.test_losses_gpu import DTYPES, F8, NINF, log_probs, logits, slots
+from tests.test_losses_gpu import DTYPES, F8, NINF, check_distill, log_probs, logits, slots
 
 pytestmark = pytest.mark.gpu
 CLASSES = [5, 9, 32, 40, 1000, 9000, 70001, 200003]      # every kernel
@@ -106,3 +106,26 @@ def test_other_classes_at_the_lowest_value(pkg, K):
         z.scatter_(1, ids.long() - 1, torch.tensor([[3.0, 1.0, -1.0]], dtype=z.dtype).expand(2, 3))
         t = torch.log(torch.tensor([[0.57, 0.285, 0.095], [0.6, 0.4, 0.1]]))
         check(pkg.distill_grads(z.cuda(), ids.cuda(), t.cuda(), tail=True, hess=True), z, ids, t, hess=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("K", CLASSES + [270001])
+def test_class_named_or_taken_near_the_lowest_value(pkg, K, dtype):
+    """Its log-probability is a number: the loss is a share of that, not infinite."""
+    rng = np.random.default_rng(K)
+    z, _ = logits(rng, 3, K, DTYPES[dtype])
+    ids, t = slots(rng, 3, K, 3, empty=0.0)
+    low = 0.8 * torch.finfo(z.dtype).min                    # its product with log2(e) is beyond 32 bits
+    z[0, ids[0, 1].long() - 1] = low
+    z[1, ids[1].long() - 1] = low                           # nothing else is named
+    z[2, ids[2, 0].long() - 1] = low / 2
+    lt = log_probs(t, 0.6)
+    check(pkg.distill_grads(z.cuda(), ids.cuda(), lt.cuda(), tail=True, hess=True), z, ids, lt, hess=True)
+    check_distill(pkg.distill_grads(z.cuda(), ids.cuda(), t.cuda(), hess=True), z, ids, t, None, 1.0, False, True)
+    a, old, adv = ids[torch.arange(3), torch.tensor([1, 0, 0])].contiguous(), torch.tensor([-1.0, -2.0, -3.0]), torch.tensor([1.0, -1.0, 0.5])
+    out = pkg.policy_grads(z.cuda(), a.cuda(), old.cuda(), adv.cuda(), hess=True)
+    loss, logp, grad, h, scale = R.policy(z, a, old, adv)
+    rel = R.part(z)
+    R.close(out[1], logp, 8 * R.U * logp.abs() + rel, "logp")
+    R.close(out[0], loss, 4 * rel * scale + R.U * loss.abs(), "loss")
+    R.close(out[2], grad, R.rounded(grad, z.dtype, 4 * rel[:, None], scale[:, None]), "grad")
