@@ -412,11 +412,12 @@ __device__ __forceinline__ bool first_slot(const Slots &s, int j) {
     return true;
 }
 // What a row's slots say by themselves, before its maximum and sum are known: the sum Q of the teacher's probabilities (1 without a tail), sum q log q,
-// the largest named prediction zn, sum q (z - zn) / tau, and (tail) sum of 2^(c (z - zn)) over the classes named, each of them once
+// the largest named prediction zn, sum q (z - zn), and (tail) sum of 2^(c (z - zn)) over the classes named, each of them once
 struct Teach { float Q, H, zn, qz, s; };
 struct alignas(16) TaughtRow { Teach teach; int flags; float tmax, r; }; // slots' flags; their largest logit, 1 / sum
 // `width` lanes share the slots; all of them get the same.  Slots without a class have id -1
 __device__ __forceinline__ Teach teach_row(const SoftArgs &a, const Slots &s, bool dup, int lane, int width) {
+    constexpr float SHARE = 1.0f / MAX_TOP; // the sum of slots that are not normalised yet stays within 32 bits when one of them does
     const float c = a.c;
     Teach o = {0.0f, 0.0f, -INFINITY, 0.0f, 0.0f};
     float tmax = -INFINITY;
@@ -429,20 +430,20 @@ __device__ __forceinline__ Teach teach_row(const SoftArgs &a, const Slots &s, bo
         const float lt = a.tail ? s.t[j] : (s.t[j] - tmax) * a.inv_tau, e = ex2(lt * LOG2E), d = s.z[j] - zn;
         s.q[j] = e;
         o.Q += e;
-        if (e != 0.0f) { o.H += e * lt; o.qz += e * (d * a.inv_tau); }
+        if (e != 0.0f) { o.H += e * lt; o.qz += e * (d * SHARE); }
         if (a.tail && (!dup || first_slot(s, j))) o.s += ex2(d * c);
     }
     o.Q = lanes_sum(o.Q, width); o.H = lanes_sum(o.H, width); o.qz = lanes_sum(o.qz, width);
-    if (a.tail) { o.s = lanes_sum(o.s, width); return o; }
+    if (a.tail) { o.s = lanes_sum(o.s, width); o.qz /= SHARE; return o; }
     const float r = 1.0f / o.Q;
     for (int j = lane; j < a.T; j += width) if (s.id[j] >= 0) s.q[j] *= r;
     o.H = o.H * r - logf(o.Q);
-    o.qz *= r;
+    o.qz *= r / SHARE;
     o.Q = 1.0f;
     return o;
 }
-// log p = y ln 2, from the difference to the row's maximum where the product with c, not that itself, is beyond 32 bits
-__device__ __forceinline__ float log_p(const SoftArgs &a, float y, float less_max) { return y == -INFINITY ? less_max * a.inv_tau : LN2 * y; }
+// tau log p = tau ln 2 y, or the difference to the row's maximum where the product with c, not that itself, is beyond 32 bits
+__device__ __forceinline__ float tau_log_p(const SoftArgs &a, float y, float less_max) { return y == -INFINITY ? less_max : LN2 * a.tau * y; }
 // r: maximum and sum of the row, less `shift`; with a tail of the classes that have no slot.  The named ones may lie anywhere then (masks leave
 // them alone, or only them): all classes together are relative to the larger of the two maxima, those without a slot among themselves to theirs.
 __device__ __forceinline__ RowOut finish_row(const SoftArgs &a, const Teach &e, Soft r, float shift, float w) {
@@ -460,16 +461,16 @@ __device__ __forceinline__ RowOut finish_row(const SoftArgs &a, const Teach &e, 
     const float ls = o.all_ls = log2f(sum);
     // the rest, when there is any: no class is left where every one is named or ruled out
     const float qt = a.tail && r.m != -INFINITY ? fmaxf(0.0f, 1.0f - e.Q) : 0.0f;
-    const float lp = log_p(a, fmaf(zn - o.all_shift, c, -o.all_M) - ls, zn - (above ? zn : zr));
-    o.loss = e.H - (e.qz + (zn == -INFINITY ? e.qz == 0.0f ? 0.0f : zn : e.Q > 0.0f ? lp * e.Q : 0.0f));
+    const float lp = tau_log_p(a, fmaf(zn - o.all_shift, c, -o.all_M) - ls, zn - (above ? zn : zr));
+    o.loss = a.tau * e.H - (e.qz + (zn == -INFINITY ? e.qz == 0.0f ? 0.0f : zn : e.Q > 0.0f ? lp * e.Q : 0.0f));
     if (zn == -INFINITY && e.Q > 0.0f) o.loss = zr == -INFINITY ? NAN : INFINITY; // nothing that the teacher names is possible
-    if (qt > 0.0f) o.loss += qt * (logf(qt) - log_p(a, part + log2f(r.s) - ls, zr - (above ? zn : zr)));
+    if (qt > 0.0f) o.loss += qt * (logf(qt) - tau_log_p(a, part + log2f(r.s) - ls, zr - (above ? zn : zr)));
     o.mass = e.Q + qt;
     o.B = r.m == -INFINITY ? 0.0f * ls : ex2(part) / sum;
     o.A = w * a.tau * (o.mass * o.B - (qt > 0.0f ? qt / r.s : 0.0f));
     o.hw = w;
     o.special = o.lp = 0.0f;
-    o.loss *= w * a.tau * a.tau;
+    o.loss *= w * a.tau; // up to here in units of the predictions, as are its largest parts
     return o;
 }
 __device__ __forceinline__ float slot_p(const SoftArgs &a, const RowOut &o, float z) { return ex2(fmaf(z - o.all_shift, a.c, -o.all_M) - o.all_ls); }
@@ -495,7 +496,10 @@ __device__ __forceinline__ RowOut class_row(const SoftArgs &a, Soft r, float shi
     // A preference adds up hundreds of them: 64 bits, and in units of the c that the terms were made with, so that roundings which all rows share
     // do not add up too
     if (KIND == ROW_LOGP) o.lp = (float)((fma((double)(t.z - shift), (double)a.c, -(double)o.M) - log2((double)r.s)) / ((double)a.c * (double)a.tau));
-    else o.lp = log_p(a, fmaf(t.z - shift, a.c, -o.M) - log2f(r.s), t.z - shift - r.m);
+    else {
+        const float y = fmaf(t.z - shift, a.c, -o.M) - log2f(r.s); // as tau_log_p
+        o.lp = y == -INFINITY ? (t.z - shift - r.m) * a.inv_tau : LN2 * y;
+    }
     o.mass = 0.0f;
     o.loss = 0.0f;
     if (KIND == ROW_POLICY) {
@@ -893,7 +897,7 @@ __global__ void __launch_bounds__(TILE) k_row_few(SoftArgs a) {
             if (DIST) {
                 const float ls = log2f(sum), lq = a.tail ? 0.0f : logf(Q), rQ = a.tail ? 1.0f : 1.0f / Q, r = 1.0f / sum;
                 if (zero != 0.0f) loss = NAN;
-                loss += entropy * rQ - (a.tail ? 0.0f : lq);
+                loss += a.tau * (entropy * rQ - (a.tail ? 0.0f : lq));
                 float qt = 0.0f, rbase = 0.0f, rr = 0.0f;
                 if (a.tail && m != -INFINITY) {
                     qt = fmaxf(0.0f, 1.0f - Q);
@@ -907,13 +911,13 @@ __global__ void __launch_bounds__(TILE) k_row_few(SoftArgs a) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     const float qk = q[k] * rQ, p = y[k] * r;
-                    if (qk != 0.0f) loss -= qk * ((z[k] - base) * a.inv_tau - LN2 * ls);
+                    if (qk != 0.0f) loss -= qk * (z[k] - base - LN2 * a.tau * ls);
                     float g = mass * p - qk;
                     if (a.tail && !(out >> k & 1u) && qt > 0.0f) g = mass * p - rr * ex2((z[k] - rbase) * c);
                     z[k] = f * g;
                     y[k] = w * p * (1.0f - p);
                 }
-                loss *= w * a.tau * a.tau;
+                loss *= w * a.tau;
             } else {
                 RowOut o;
 #pragma unroll

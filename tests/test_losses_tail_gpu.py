@@ -129,3 +129,17 @@ def test_class_named_or_taken_near_the_lowest_value(pkg, K, dtype):
     R.close(out[1], logp, 8 * R.U * logp.abs() + rel, "logp")
     R.close(out[0], loss, 4 * rel * scale + R.U * loss.abs(), "loss")
     R.close(out[2], grad, R.rounded(grad, z.dtype, 4 * rel[:, None], scale[:, None]), "grad")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("K", CLASSES[1:])
+@pytest.mark.parametrize("tau", [0.5, 1.0, 2.0])
+def test_many_named_classes_near_the_lowest_value(pkg, K, dtype, tau):
+    """What the slots add up to before they are divided by their sum, and what a temperature divides, may be beyond 32 bits where the loss is not."""
+    rng = np.random.default_rng(K)
+    z, _ = logits(rng, 2, K, DTYPES[dtype])
+    ids, _ = slots(rng, 2, K, 7, empty=0.0)
+    z.scatter_(1, ids[:, 1:].long() - 1, 0.8 * torch.finfo(z.dtype).min)
+    t = torch.zeros((2, 7))
+    t[:, 1:] = tau * float(np.log(0.25))                    # the masked six have 0.6 together
+    check_distill(pkg.distill_grads(z.cuda(), ids.cuda(), t.cuda(), tau=tau, hess=True), z, ids, t, None, tau, False, True)
