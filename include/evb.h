@@ -409,7 +409,7 @@ EVB_API int32_t evb_hist_rows_noalloc(int32_t device, void *stream, const uint8_
  *   grad     device, type of z, row i at grad + i * ldg, or NULL: derivatives of the sum of the losses by z.  All K entries of all n rows
  *            are written.  It must not overlap z
  *   hess     the same for the second derivatives' positive part: w p_k (1 - p_k), divided by tau^2 for the policy loss; or NULL
- *   class codes are 1..K; 0 names no class.  A row that names a class above K gets NaN in all its outputs.
+ *   class codes are 1..K; 0 names no class.  A row that counts and names a class above K gets NaN in all its outputs.
  * The calls enqueue their kernels on `stream` (cudaStream_t) and return; they allocate nothing and can be captured into a CUDA graph.  The
  * calling thread's current device stays what it was.  Sums and probabilities are 32-bit floats whatever the type of z, sums of log
  * ratios 64-bit ones; results do not depend on scheduling: equal calls give equal bits.
@@ -436,7 +436,8 @@ EVB_API int32_t evb_hist_rows_noalloc(int32_t device, void *stream, const uint8_
  * evb_preference_grads -- preferences between sequences of rows by their log ratios.
  *   label    device uint32 [n]: the class of every row, 0 = not counted (a prompt, padding)
  *   seq      device int32 [2 pairs + 1] ascending within 0..n: sequence s is rows seq[s] .. seq[s + 1] - 1; pair p prefers sequence 2 p to
- *            sequence 2 p + 1.  Rows outside of all sequences have zero gradients
+ *            sequence 2 p + 1.  Rows outside of all sequences, and of pairs of weight 0, have zero gradients, whatever their labels (a label above
+ *            K makes NaN of its logp and of its pair's margin there too)
  *   ref_logp device float [n]: the reference's log-probabilities, or NULL for zeros;  w  device float [pairs] or NULL
  *            D_s = sum over its rows of (log p_label - ref_logp), divided by their number when mean != 0;  m = beta (D_2p - D_2p+1)
  *            loss = w ((1 - smooth) softplus(-m) + smooth softplus(m));  grad as it follows from that (tau = 1)
