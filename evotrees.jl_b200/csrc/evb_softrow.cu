@@ -72,7 +72,8 @@ struct Soft { float m, s; };
 __device__ __forceinline__ float base_of(float m, float c) { const float M = __fmul_rn(m, c); return M == -INFINITY ? 0.0f : M; } // nothing seen: every term is 2^-inf
 __device__ __forceinline__ float rise(float m, float c, float base) { return __fmul_rn(m, c) - base; } // between two M: the product rounded, never a multiply-add
 // Where M's rounding would reach the exponents, or the products overflow (masks are often made of the type's lowest value), a part of a row
-// sees nothing: its terms are 2^-inf.  When that is the largest prediction of the whole row, it is looked at again, less its maximum.
+// sees nothing: its terms are 2^-inf.  When that is the largest prediction of the whole row (with a tail: of the classes without a slot), it is
+// looked at again, less its maximum.
 __device__ __forceinline__ bool is_far(float m, float c) { return fabsf(m) * c > 1.0e9f && m != -INFINITY; }
 
 struct RowLoss { float loss, d; }; // loss and its derivative by log p of the class taken
@@ -600,8 +601,9 @@ __device__ __forceinline__ int put_into(const SoftArgs &a, const RowAt<ZT> &at, 
 
 // Rows of up to V granules for each of G lanes (a power of two up to 32): 32 / G rows a warp, 8 warps a CTA.
 template <typename ZT, int KIND, int V>
-// The row stays in registers between its two uses.  Measured: policy 20011 x 1000 f32 34 us (floor 24), 100k x 200 f32 with ten slots 65 (26): there
-// most instructions are the slots' (12000 of a row's threads together, of which the 200 classes take 2000).
+// The row stays in registers between its two uses.  Measured: policy 20011 x 1000 f32 34 us (floor 24), 100k x 200 f32 with ten slots 66 (26).  At 200
+// classes four rows share a warp, which takes 840 instructions for a policy (39 us), 1340 with one slot (57), 1520 with ten (66), 1870 with 32 (84):
+// what slots cost is mostly the same however many there are, their loops and sums over lanes.  The issue slots are 59 % used, with 22 warps an SM (80 registers).
 __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words) {
     extern __shared__ __align__(16) unsigned char s_raw[];
     constexpr int E = Pack<ZT>::E;
@@ -682,7 +684,7 @@ __global__ void __launch_bounds__(256) k_row_lanes(SoftArgs a, int G, int words)
 
 // Rows of up to 32 classes: a thread per row, 128 rows a CTA, all that they hold staged through shared memory so that memory is read and written
 // in order.  Rows of shared memory are an odd number of words apart: neighbours fall into different banks.
-// Policy 1M x 18 with hessians: 52 us (floor 37).
+// Policy 1M x 18 with hessians: 52 us (floor 37): shared memory is busy for 82 % of them, 1110 instructions a row.
 constexpr int TILE = 128, TILE_K = 32, TILE_T = 32;
 struct TileGeom { int Kp, Tp; uint32_t by_K, by_T; }; // by_*: (c * by) >> 32 is c / K (c / T) for c < 2^13
 template <typename T, typename F>
@@ -832,7 +834,7 @@ __global__ void __launch_bounds__(TILE) k_row_tile(SoftArgs a, TileGeom ge) {
 
 // The same for 2 to 8 classes of 32 bits, their number known to the compiler: a row's predictions stay in registers, read by their thread alone (the
 // rows of a warp are neighbours: what one thread leaves of a line, others take); gradients and hessians go out through shared memory.
-// 2M x 5 with three slots and hessians: 65 us (floor 28); k_row_tile takes 100, 1400 instructions a row.
+// 2M x 5 with three slots and hessians: 65 us (floor 28), 845 instructions a row that use 77 % of the issue slots; k_row_tile takes 100 us and 1400.
 template <int KIND, int K>
 __global__ void __launch_bounds__(TILE) k_row_few(SoftArgs a) {
     extern __shared__ __align__(16) float s_tile[]; // gradients [TILE][K], hessians
@@ -1005,7 +1007,7 @@ __device__ __forceinline__ bool table_has(int *table, int places, int id) {
 // in hand: eight granules a thread at 64 registers, 1024 threads.  Measured and left: rows that a CTA stays for, fetched ahead by bulk
 // copies into a ring (2.4 to 3.0 TB/s instead of 4.2); independent warps in two passes, the second out of L2 (2.1); a warp more for the slots
 // (three CTAs an SM instead of four: 770 us instead of 597).  4.9 TB/s for 8192 x 65537 bf16 (420 us, floor 316).
-// PRE: k_row_taught has seen to the slots (4096 x 131072 bf16 with 64 and a tail: 523 us, floor 322; 597 without).
+// PRE: k_row_taught has seen to the slots (4096 x 131072 bf16 with 64 and a tail: 528 us, floor 322; 597 without).
 template <typename ZT, int KIND, int V, int NT, bool PRE = false>
 __global__ void __launch_bounds__(NT, (V == 16 ? 512 : 1024) / NT) k_row_ctas(SoftArgs a, int lcs, int words) {
     extern __shared__ __align__(16) unsigned char s_raw[];
@@ -1526,6 +1528,9 @@ int32_t launch_typed(SoftArgs a, int sms, cudaStream_t st, void *work) {
     }
     lcs = 0;
     while (lcs < 3 && !holds(256, 8)) ++lcs;
+    // Above 131072 classes of 16 bits, 65536 of 32 bits, eight CTAs of 512 threads, two an SM.  Microseconds against k_row_walk, 1000 rows: policy 140001 bf16
+    // 193 and 152, 200003 225 and 217, 262136 250 and 279, 131064 f32 218 and 275 (300 rows x 200003 bf16: 76 and 95), so of many rows the walk
+    // is as good or better up to some 200000 classes of 16 bits.  It is also better without gradients (200003 bf16: 168 and 92) and with a tail (301 and 223)
     if (holds(512, 8) && (a.n << lcs) <= 0x7fffffff) {
         if constexpr (KIND == ROW_DISTILL) {
             if (work) {
