@@ -464,7 +464,7 @@ __device__ __forceinline__ RowOut finish_row(const SoftArgs &a, const Teach &e, 
     const float qt = a.tail && r.m != -INFINITY ? fmaxf(0.0f, 1.0f - e.Q) : 0.0f;
     const float lp = tau_log_p(a, fmaf(zn - o.all_shift, c, -o.all_M) - ls, zn - (above ? zn : zr));
     o.loss = a.tau * e.H - (e.qz + (zn == -INFINITY ? e.qz == 0.0f ? 0.0f : zn : e.Q > 0.0f ? lp * e.Q : 0.0f));
-    if (zn == -INFINITY && e.Q > 0.0f) o.loss = zr == -INFINITY ? NAN : INFINITY; // nothing that the teacher names is possible
+    if (zn == -INFINITY && e.Q > 0.0f) o.loss = isfinite(ls) ? INFINITY : NAN; // nothing that the teacher names is possible; or they are NaN, or all is ruled out
     if (qt > 0.0f) o.loss += qt * (logf(qt) - tau_log_p(a, part + log2f(r.s) - ls, zr - (above ? zn : zr)));
     o.mass = e.Q + qt;
     o.B = r.m == -INFINITY ? 0.0f * ls : ex2(part) / sum;

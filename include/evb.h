@@ -409,7 +409,8 @@ EVB_API int32_t evb_hist_rows_noalloc(int32_t device, void *stream, const uint8_
  *   grad     device, type of z, row i at grad + i * ldg, or NULL: derivatives of the sum of the losses by z.  All K entries of all n rows
  *            are written.  It must not overlap z
  *   hess     the same for the second derivatives' positive part: w p_k (1 - p_k), divided by tau^2 for the policy loss; or NULL
- *   class codes are 1..K; 0 names no class.  A row that counts and names a class above K gets NaN in all its outputs.
+ *   class codes are 1..K; 0 names no class.  A row that counts and names a class above K gets NaN in all its outputs,
+ *            and so does one that holds NaN or +inf.  -inf and the type's lowest value rule a class out
  * The calls enqueue their kernels on `stream` (cudaStream_t) and return; they allocate nothing and can be captured into a CUDA graph.  The
  * calling thread's current device stays what it was.  Sums and probabilities are 32-bit floats whatever the type of z, sums of log
  * ratios 64-bit ones; results do not depend on scheduling: equal calls give equal bits.

@@ -143,3 +143,19 @@ def test_many_named_classes_near_the_lowest_value(pkg, K, dtype, tau):
     t = torch.zeros((2, 7))
     t[:, 1:] = tau * float(np.log(0.25))                    # the masked six have 0.6 together
     check_distill(pkg.distill_grads(z.cuda(), ids.cuda(), t.cuda(), tau=tau, hess=True), z, ids, t, None, tau, False, True)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("K", CLASSES)
+@pytest.mark.parametrize("tail", [False, True])
+def test_rows_with_a_prediction_that_is_no_number(pkg, K, tail, value):
+    """Wherever it is, in a slot or not, the only one named or not: NaN in all that the row gives."""
+    for dtype in DTYPES.values():
+        z = torch.zeros((4, K), dtype=dtype)
+        z[0, 1], z[1, 2], z[2, K - 1] = value, value, value
+        ids = torch.tensor([[2, 0], [1, 3], [1, 2], [1, 2]], dtype=torch.int32)
+        out = pkg.distill_grads(z.cuda(), ids.cuda(), torch.full((4, 2), -0.8).cuda(), tail=tail, hess=True)
+        assert all(torch.isnan(o[:3]).all() and torch.isfinite(o[3]).all() for o in out)
+        a, v = torch.tensor([2, 1, 1, 1], dtype=torch.int32).cuda(), torch.ones(4, device="cuda")
+        out = pkg.policy_grads(z.cuda(), a, -v, v, hess=True)
+        assert all(torch.isnan(o[:3]).all() and torch.isfinite(o[3]).all() for o in out)
